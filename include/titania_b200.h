@@ -59,6 +59,8 @@ typedef struct tb200_weight tb200_weight; /* Device::Weight, bf16 (model/device.
 typedef struct tb200_model tb200_model;   /* fused-path model (no trait counterpart) */
 typedef struct tb200_state tb200_state;   /* fused-path State (model/model.rs:156-172) */
 typedef struct tb200_tp tb200_tp;         /* a tensor-parallel group (one rank per process and GPU) */
+typedef struct tb200_q8 tb200_q8;         /* rows of 8-bit integers with an f32 scale each */
+typedef struct tb200_scorer tb200_scorer; /* log probabilities of given tokens */
 typedef struct tb200_sampler tb200_sampler; /* top-k / top-p / temperature sampling state on the device */
 
 /* Message for the last nonzero return on this thread. */
@@ -135,6 +137,11 @@ TB200_API int tb200_alloc(tb200_device* dev, size_t len, tb200_buffer** out);
 TB200_API int tb200_resize(tb200_device* dev, tb200_buffer* buf, size_t len);
 /* The buffer's current length (Vec::len of `read`'s result). */
 TB200_API size_t tb200_buffer_len(const tb200_buffer* buf);
+/* The buffer's device address (NULL for an empty one), valid until the buffer
+ * is freed: for callers that fill or read it with kernels of their own, in
+ * order with the device's stream (tb200_device_stream). No counterpart in the
+ * reference. */
+TB200_API float* tb200_buffer_data(const tb200_buffer* buf);
 /* device.rs:29 `read(&self, &Buffer) -> Vec<f32>`; `len` must equal the
  * buffer's length. Waits for the device. */
 TB200_API int tb200_read(tb200_device* dev, const tb200_buffer* buf, float* out, size_t len);
@@ -172,6 +179,63 @@ TB200_API int tb200_attention_cache(tb200_device* dev, tb200_buffer* out, const 
                                     const tb200_weight* cache, const size_t* positions, size_t batch, size_t n_heads);
 /* device.rs:88 `silu_mul(&self, gate, up)`. */
 TB200_API int tb200_silu_mul(tb200_device* dev, tb200_buffer* gate, const tb200_buffer* up);
+
+/* ---- 8-bit rows (no counterpart in the reference) -------------------------- */
+
+/* Rows of 8-bit integers, each with an f32 scale: value [r][c] stands for
+ * values[r][c] * scales[r]. Activations (a row and scale per token) and
+ * weights (a row and scale per output channel) are both held so; tb200_matmul_q8
+ * multiplies the two. Everything below is enqueued on the device's stream and
+ * returns without waiting, unless it says otherwise; no call but the ones
+ * that make a handle allocates memory, so calls can be captured into a CUDA
+ * graph on that stream. A call with no rows does nothing.
+ *
+ * How values become integers, everywhere here: with m the largest magnitude
+ * of a row's values, the scale is m / 127 rounded to f32, and each integer is
+ * the value divided by that scale, rounded to nearest (ties to even) in 64-bit
+ * arithmetic, at most 127 in magnitude. A row of zeros (or whose scale rounds
+ * to zero) has scale 0 and zeros. A row with a NaN or an infinity, or
+ * whose scale f32 does not hold, has scale NaN and zeros: every product with
+ * it is NaN. */
+
+/* A handle of `rows` (0 or more) rows of `cols` (1 .. 2^31 - 1) values, all zero. */
+TB200_API int tb200_q8_new(tb200_device* dev, size_t rows, size_t cols, tb200_q8** out);
+TB200_API int tb200_q8_free(tb200_device* dev, tb200_q8* q);
+/* Changes the number of rows, up to the number it was made with; what the
+ * rows hold stays (tb200_resize for this kind of handle). */
+TB200_API int tb200_q8_resize(tb200_device* dev, tb200_q8* q, size_t rows);
+TB200_API int tb200_q8_shape(const tb200_q8* q, size_t* rows, size_t* cols);
+/* Copies the integers ([rows][cols]) and scales ([rows]) to the host; waits. */
+TB200_API int tb200_q8_read(tb200_device* dev, const tb200_q8* q, int8_t* values, float* scales);
+/* Sets them from the host (weights that were quantised elsewhere; every int8
+ * value is allowed); waits. */
+TB200_API int tb200_q8_write(tb200_device* dev, tb200_q8* q, const int8_t* values, const float* scales);
+/* Device addresses: row r of the integers starts at *values + r * *ld bytes.
+ * The ld - cols bytes between rows are zeros and have to stay so. */
+TB200_API int tb200_q8_data(const tb200_q8* q, int8_t** values, size_t* ld, float** scales);
+
+/* out = x in 8 bits: x holds rows * cols values. */
+TB200_API int tb200_quantize(tb200_device* dev, tb200_q8* out, const tb200_buffer* x);
+/* A handle with the bf16 matrix `w` in 8 bits, a scale for each of its rows
+ * (output channels); enqueued, so `w` must not be freed before the next call
+ * that waits (tb200_free_weight does). */
+TB200_API int tb200_quantize_weight(tb200_device* dev, const tb200_weight* w, tb200_q8** out);
+/* out = the values that x stands for, integer * scale in f32. */
+TB200_API int tb200_dequantize(tb200_device* dev, tb200_buffer* out, const tb200_q8* x);
+/* tb200_add and tb200_rmsnorm with the output in 8 bits, in one pass:
+ * x += y (where y is not NULL; tb200_add's f32 sums), then per row of `cols`
+ * values h = x[t]: out[t] = h * w / sqrt(mean(h^2) + eps) in 8 bits, the mean
+ * and the norm in 64-bit arithmetic. x and y hold rows * cols values, w cols;
+ * eps is not negative. x itself is not normalised. */
+TB200_API int tb200_add_rmsnorm_q8(tb200_device* dev, tb200_q8* out, tb200_buffer* x, const tb200_buffer* y,
+                                   const tb200_weight* w, float eps);
+/* out[t][c] = (sum over k of w[c][k] * x[t][k]) * (w.scale[c] * x.scale[t]):
+ * tb200_matmul over 8-bit rows. The sum of integer products is exact (32-bit
+ * integers; up to 131071 columns), its f32 value is then multiplied by the f32
+ * product of the scales. out holds x.rows * w.rows values. An error inside
+ * the kernel (a wait that timed out) is reported by the next call that waits
+ * (tb200_sync, tb200_read). */
+TB200_API int tb200_matmul_q8(tb200_device* dev, tb200_buffer* out, const tb200_q8* w, const tb200_q8* x);
 
 /* The trait has no free (handles live as long as the process, as with
  * Titania, model/titania.rs:43-55); these let a caller give memory back. */
@@ -410,6 +474,40 @@ TB200_API int tb200_sample(tb200_sampler* sampler, const tb200_buffer* logits, u
 TB200_API int tb200_sample_enqueue(tb200_sampler* sampler, const tb200_buffer* logits);
 /* The generator states, rows x u64 (sampler.rs:63-77's Rng). */
 TB200_API int tb200_sampler_state(tb200_sampler* sampler, uint64_t* out);
+
+/* ---- log probabilities (no counterpart in the reference) ------------------- */
+
+/* What a scorer holds: room for `rows` rows of results over logits of
+ * `vocab` values (1 .. 2^31 - 1), and the `top` (0 .. 64, at most vocab)
+ * most likely alternatives of each. */
+TB200_API int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, tb200_scorer** out);
+TB200_API int tb200_scorer_free(tb200_scorer* s);
+/* For each of the first n rows of `logits` ([n][vocab] f32, the buffer at least
+ * that long; n <= rows), with p = softmax(row):
+ *   logprob[i]       ln p[tokens[i]];
+ *   entropy[i]       -sum p ln p, in nats (tokens of probability 0 add 0);
+ *   top_ids[i]       the `top` largest logits' ids, largest first, in
+ *                    tb200_argmax's order: ties go to the lowest id;
+ *   top_logprobs[i]  their log probabilities.
+ * A logit of -inf (a token that is excluded) has log probability -inf. A row
+ * with a NaN or +inf, or with nothing but -inf, has NaN throughout (its
+ * top_ids are in order all the same). `tokens` is host memory (copied before
+ * the call returns, except page-locked memory, which must stay as it is until
+ * the work is done) or memory of this device, read on the device's stream. A
+ * token id past the vocabulary is an error in host memory; in device
+ * memory, where the call cannot see it, its log probability is NaN. The
+ * results stay on the device (tb200_scorer_data), those of rows n and up as
+ * they were; nothing is allocated and nothing waits. Calls on one scorer share
+ * its workspace: their work must not overlap. In a captured call `tokens` must
+ * be device memory. */
+TB200_API int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint32_t* tokens, size_t n);
+/* The same, then copies the results to the host (n, n, [n][top], [n][top];
+ * each may be NULL) and waits. */
+TB200_API int tb200_score(tb200_scorer* s, const tb200_buffer* logits, const uint32_t* tokens, size_t n,
+                          float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
+/* Device addresses of the results: [rows], [rows], [rows][top], [rows][top]. */
+TB200_API int tb200_scorer_data(const tb200_scorer* s, float** logprob, float** entropy, uint32_t** top_ids,
+                                float** top_logprobs);
 
 /* ---- tracing ------------------------------------------------------------ */
 

@@ -49,6 +49,7 @@ P = ctypes.c_void_p
 SZ = ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
 F32P = ctypes.POINTER(ctypes.c_float)
+I8P = ctypes.POINTER(ctypes.c_int8)
 U16P = ctypes.POINTER(ctypes.c_uint16)
 U32P = ctypes.POINTER(ctypes.c_uint32)
 SZP = ctypes.POINTER(ctypes.c_size_t)
@@ -74,6 +75,7 @@ SIGNATURES = {
     "tb200_alloc": (ctypes.c_int, [P, SZ, PP]),
     "tb200_resize": (ctypes.c_int, [P, P, SZ]),
     "tb200_buffer_len": (ctypes.c_size_t, [P]),
+    "tb200_buffer_data": (ctypes.c_void_p, [P]),
     "tb200_read": (ctypes.c_int, [P, P, F32P, SZ]),
     "tb200_write": (ctypes.c_int, [P, P, F32P, SZ]),
     "tb200_copy": (ctypes.c_int, [P, P, SZ, P, SZ, SZ]),
@@ -85,6 +87,18 @@ SIGNATURES = {
     "tb200_attention": (ctypes.c_int, [P, P, P, P, P, SZ, SZ, SZ, SZ]),
     "tb200_attention_cache": (ctypes.c_int, [P, P, P, P, SZP, SZ, SZ]),
     "tb200_silu_mul": (ctypes.c_int, [P, P, P]),
+    "tb200_q8_new": (ctypes.c_int, [P, SZ, SZ, PP]),
+    "tb200_q8_free": (ctypes.c_int, [P, P]),
+    "tb200_q8_resize": (ctypes.c_int, [P, P, SZ]),
+    "tb200_q8_shape": (ctypes.c_int, [P, SZP, SZP]),
+    "tb200_q8_read": (ctypes.c_int, [P, P, I8P, F32P]),
+    "tb200_q8_write": (ctypes.c_int, [P, P, I8P, F32P]),
+    "tb200_q8_data": (ctypes.c_int, [P, PP, SZP, PP]),
+    "tb200_quantize": (ctypes.c_int, [P, P, P]),
+    "tb200_quantize_weight": (ctypes.c_int, [P, P, PP]),
+    "tb200_dequantize": (ctypes.c_int, [P, P, P]),
+    "tb200_add_rmsnorm_q8": (ctypes.c_int, [P, P, P, P, P, ctypes.c_float]),
+    "tb200_matmul_q8": (ctypes.c_int, [P, P, P, P]),
     "tb200_free_buffer": (ctypes.c_int, [P, P]),
     "tb200_free_weight": (ctypes.c_int, [P, P]),
     "tb200_argmax": (ctypes.c_int, [P, P, U32P]),
@@ -95,6 +109,11 @@ SIGNATURES = {
     "tb200_sample": (ctypes.c_int, [P, P, U32P]),
     "tb200_sample_enqueue": (ctypes.c_int, [P, P]),
     "tb200_sampler_state": (ctypes.c_int, [P, ctypes.POINTER(ctypes.c_uint64)]),
+    "tb200_scorer_new": (ctypes.c_int, [P, SZ, SZ, SZ, PP]),
+    "tb200_scorer_free": (ctypes.c_int, [P]),
+    "tb200_score_enqueue": (ctypes.c_int, [P, P, P, SZ]),
+    "tb200_score": (ctypes.c_int, [P, P, P, SZ, F32P, F32P, U32P, F32P]),
+    "tb200_scorer_data": (ctypes.c_int, [P, PP, PP, PP, PP]),
     "tb200_model_create": (ctypes.c_int, [P, ctypes.POINTER(Config), PP]),
     "tb200_model_bind": (ctypes.c_int, [P, ctypes.c_char_p, P]),
     "tb200_model_finalize": (ctypes.c_int, [P]),

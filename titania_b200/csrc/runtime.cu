@@ -42,6 +42,14 @@ int use(tb200_device* d) {
   return TB200_OK;
 }
 
+int settle(tb200_device* d) {
+  CUDA_TRY(cudaStreamSynchronize(d->stream));
+  volatile int* e = d->async_err;
+  if (!*e) return TB200_OK;
+  *e = 0;
+  return fail(TB200_ERR_TIMEOUT, "a wait inside an 8-bit contraction timed out; its output is not complete");
+}
+
 // model.rs:239-250, on the host exactly as the reference computes it.
 std::vector<float> rope_table(size_t max_len, size_t head_dim, float theta) {
   size_t half = head_dim / 2;
@@ -156,9 +164,13 @@ int tb200_device_open(int ordinal, tb200_device** out) {
   if (e == cudaSuccess) e = cudaMalloc(&d->best, sizeof(unsigned long long));
   if (e == cudaSuccess) e = cudaMalloc(&d->err, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(d->err, 0, sizeof(int));
+  if (e == cudaSuccess) e = cudaHostAlloc(&d->async_err, sizeof(int), cudaHostAllocMapped);
+  if (e == cudaSuccess) *d->async_err = 0;
+  if (e == cudaSuccess) e = cudaHostGetDevicePointer(&d->async_err_dev, d->async_err, 0);
   if (e != cudaSuccess) {
     cudaFree(d->best);
     cudaFree(d->err);
+    if (d->async_err) cudaFreeHost(d->async_err);
     delete d;
     return fail(TB200_ERR_CUDA, std::string("device setup: ") + cudaGetErrorString(e));
   }
@@ -175,6 +187,7 @@ int tb200_device_close(tb200_device* d) {
   cudaFree(d->best);
   cudaFree(d->split);
   cudaFree(d->err);
+  cudaFreeHost(d->async_err);
   cudaFree(d->ao_part);
   cudaFree(d->ao_ticket);
   cudaFree(d->ao_meta);
@@ -187,8 +200,7 @@ int tb200_device_close(tb200_device* d) {
 
 int tb200_sync(tb200_device* d) {
   if (int rc = use(d)) return rc;
-  CUDA_TRY(cudaStreamSynchronize(d->stream));
-  return TB200_OK;
+  return rt::settle(d);
 }
 
 void* tb200_device_stream(tb200_device* d) { return d ? static_cast<void*>(d->stream) : nullptr; }
@@ -254,14 +266,14 @@ int tb200_resize(tb200_device* d, tb200_buffer* b, size_t len) {
 }
 
 size_t tb200_buffer_len(const tb200_buffer* b) { return b ? b->len : 0; }
+float* tb200_buffer_data(const tb200_buffer* b) { return b ? b->ptr : nullptr; }
 
 int tb200_read(tb200_device* d, const tb200_buffer* b, float* out, size_t len) {
   if (int rc = use(d)) return rc;
   ARG_CHECK(b && (out || len == 0), "null argument");
   ARG_CHECK(len == b->len, "read: buffer holds " + std::to_string(b->len) + " activations, not " + std::to_string(len));
   if (len) CUDA_TRY(cudaMemcpyAsync(out, b->ptr, len * 4, cudaMemcpyDeviceToHost, d->stream));
-  CUDA_TRY(cudaStreamSynchronize(d->stream));
-  return TB200_OK;
+  return rt::settle(d);
 }
 
 // titania.rs:133-137

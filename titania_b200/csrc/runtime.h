@@ -45,6 +45,11 @@ struct tb200_device {
   const void* ao_map_base = nullptr;  // the cache the tensor map describes
   size_t ao_map_rows = 0;
   CUtensorMap ao_map{};
+  // Error word of the operators that return before their kernels have run
+  // (matmul_q8): page-locked and mapped, so that a call which waits for the
+  // device reads it without a copy (rt::settle).
+  int* async_err = nullptr;      // host address
+  int* async_err_dev = nullptr;  // the same word as kernels see it
 };
 
 struct tb200_buffer {
@@ -58,6 +63,16 @@ struct tb200_weight {
   size_t numel = 0;
   bool has_map = false;
   CUtensorMap map{};  // operand map of a matrix for the tensor-core contraction
+};
+
+// Rows of 8-bit integers with one f32 scale each: row r, column c stands for
+// values[r * ld + c] * scales[r]. Activations (a row per token) and weights (a
+// row per output channel) are both of this kind (q8.cu, q8_gemm.cu).
+struct tb200_q8 {
+  int8_t* values = nullptr;  // [cap][ld]
+  float* scales = nullptr;   // [cap]
+  size_t rows = 0, cap = 0, cols = 0;
+  size_t ld = 0;  // cols rounded up to 16 bytes; the padding holds zeros
 };
 
 struct FusedLayer {
@@ -174,6 +189,9 @@ int fail(int code, const std::string& msg);
 int launched(const char* what);
 // Makes `d` the current device.
 int use(tb200_device* d);
+// Waits for the device's stream and reports an error that a kernel left in
+// async_err since the last such call.
+int settle(tb200_device* d);
 // model.rs:239-250, on the host.
 std::vector<float> rope_table(size_t max_len, size_t head_dim, float theta);
 const char* last_error();

@@ -46,6 +46,25 @@ class Weight:
         self._h = None
 
 
+class DeviceArray:
+    """A handle's device memory as other libraries see it (the CUDA array
+    interface: `torch.as_tensor(array, device="cuda")` shares it). It is valid
+    while the handle is; work on it has to be ordered with the device's stream
+    (`B200.stream`), which the interface names."""
+
+    __slots__ = ("__cuda_array_interface__", "_owner")
+
+    def __init__(self, owner, dev, ptr, shape, typestr, strides=None):
+        self._owner = owner  # the memory lives as long as its handle
+        self.__cuda_array_interface__ = {"shape": tuple(int(n) for n in shape), "typestr": typestr,
+                                         "data": (int(ptr or 0), False), "version": 3, "strides": strides,
+                                         "stream": dev.stream}
+
+    @property
+    def shape(self):
+        return self.__cuda_array_interface__["shape"]
+
+
 class Buffer:
     """Device::Buffer: f32 activations in device memory."""
 
@@ -57,9 +76,53 @@ class Buffer:
     def __len__(self):
         return int(lib().tb200_buffer_len(self._h))
 
+    @property
+    def __cuda_array_interface__(self):
+        return DeviceArray(self, self._dev, lib().tb200_buffer_data(self._h), (len(self),), "<f4").__cuda_array_interface__
+
     def __del__(self):
         if self._h and self._dev is not None and self._dev._h and not sys.is_finalizing():
             lib().tb200_free_buffer(self._dev._h, self._h)
+        self._h = None
+
+
+class Q8:
+    """Rows of 8-bit integers in device memory, each with an f32 scale: row r,
+    column c stands for values[r, c] * scales[r]. Activations have a row per
+    token, weights one per output channel."""
+
+    __slots__ = ("_h", "_dev", "cols")
+
+    def __init__(self, handle, dev):
+        self._h, self._dev = handle, dev
+        self.cols = self.shape[1]
+
+    @property
+    def shape(self) -> tuple:
+        rows, cols = ctypes.c_size_t(), ctypes.c_size_t()
+        call("tb200_q8_shape", self._h, ctypes.byref(rows), ctypes.byref(cols))
+        return int(rows.value), int(cols.value)
+
+    def _data(self):
+        v, ld, s = ctypes.c_void_p(), ctypes.c_size_t(), ctypes.c_void_p()
+        call("tb200_q8_data", self._h, ctypes.byref(v), ctypes.byref(ld), ctypes.byref(s))
+        return v.value, int(ld.value), s.value
+
+    @property
+    def values(self) -> DeviceArray:
+        """The integers on the device, [rows, cols] int8 (rows lie a multiple
+        of 16 bytes apart; the bytes between them have to stay zero)."""
+        v, ld, _ = self._data()
+        return DeviceArray(self, self._dev, v, self.shape, "|i1", (ld, 1))
+
+    @property
+    def scales(self) -> DeviceArray:
+        """The scales on the device, [rows] f32."""
+        return DeviceArray(self, self._dev, self._data()[2], self.shape[:1], "<f4")
+
+    def __del__(self):
+        if self._h and self._dev is not None and self._dev._h and not sys.is_finalizing():
+            lib().tb200_q8_free(self._dev._h, self._h)
         self._h = None
 
 
@@ -199,6 +262,59 @@ class B200:
     def silu_mul(self, gate: Buffer, up: Buffer) -> None:
         call("tb200_silu_mul", self._h, gate._h, up._h)
 
+    # ---- 8-bit rows -----------------------------------------------------------
+
+    def q8(self, rows: int, cols: int) -> Q8:
+        """`rows` rows of `cols` zeros in 8 bits, with scales of zero."""
+        h = ctypes.c_void_p()
+        call("tb200_q8_new", self._h, int(rows), int(cols), ctypes.byref(h))
+        return Q8(h.value, self)
+
+    def resize_q8(self, q: Q8, rows: int) -> None:
+        """`resize` for 8-bit rows: at most the number they were made with."""
+        call("tb200_q8_resize", self._h, q._h, int(rows))
+
+    def read_q8(self, q: Q8):
+        """(integers [rows, cols] int8, scales [rows] f32) on the host; waits."""
+        rows, cols = q.shape
+        v, s = np.empty((rows, cols), dtype=np.int8), np.empty(rows, dtype=np.float32)
+        call("tb200_q8_read", self._h, q._h, v.ctypes.data_as(_lib.I8P), s.ctypes.data_as(_lib.F32P))
+        return v, s
+
+    def write_q8(self, q: Q8, values, scales) -> None:
+        """Sets integers and scales from the host; waits."""
+        v, s = np.ascontiguousarray(values), np.ascontiguousarray(scales, dtype=np.float32)
+        if v.dtype != np.int8 or v.shape != q.shape or s.shape != q.shape[:1]:
+            raise ValueError(f"8-bit rows of shape {q.shape} given {v.dtype} values of shape {v.shape} and "
+                             f"scales of shape {s.shape}")
+        call("tb200_q8_write", self._h, q._h, v.ctypes.data_as(_lib.I8P), s.ctypes.data_as(_lib.F32P))
+
+    def quantize(self, out: Q8, x: Buffer) -> None:
+        """out = the rows of x in 8 bits: per row, scale = max|x| / 127 and
+        integers = x / scale rounded to nearest."""
+        call("tb200_quantize", self._h, out._h, x._h)
+
+    def quantize_weight(self, w: Weight) -> Q8:
+        """A bf16 matrix in 8 bits with a scale per row (output channel)."""
+        h = ctypes.c_void_p()
+        call("tb200_quantize_weight", self._h, w._h, ctypes.byref(h))
+        return Q8(h.value, self)
+
+    def dequantize(self, out: Buffer, x: Q8) -> None:
+        """out = the values that x stands for: integer * scale."""
+        call("tb200_dequantize", self._h, out._h, x._h)
+
+    def add_rmsnorm_q8(self, out: Q8, x: Buffer, y: Buffer | None, weight: Weight, eps: float) -> None:
+        """`add` and `rmsnorm` with the output in 8 bits: x += y (unless y is
+        None), then out = the rows of rmsnorm(x, weight) in 8 bits with a scale
+        per token. x keeps the sum."""
+        call("tb200_add_rmsnorm_q8", self._h, out._h, x._h, None if y is None else y._h, weight._h, eps)
+
+    def matmul_q8(self, out: Buffer, w: Q8, x: Q8) -> None:
+        """`matmul` over 8-bit rows: out[t] = w · x[t], the integers' sums exact,
+        times the scales of the channel and the token."""
+        call("tb200_matmul_q8", self._h, out._h, w._h, x._h)
+
     # ---- beyond the trait ---------------------------------------------------
 
     def argmax(self, logits: Buffer) -> int:
@@ -218,4 +334,4 @@ class B200:
              int(n_heads))
 
 
-__all__ = ["B200", "Buffer", "Weight", "Tensor", "DeviceError"]
+__all__ = ["B200", "Buffer", "DeviceArray", "Q8", "Weight", "Tensor", "DeviceError"]

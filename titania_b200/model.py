@@ -22,7 +22,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import call
-from .device import B200, Tensor
+from .device import B200, DeviceArray, Tensor
 
 BATCH = 64  # model/model.rs:8
 
@@ -167,52 +167,101 @@ class OpState:
         self.k_cache = [d.alloc(max_len * kv_dim) for _ in range(c.num_hidden_layers)]
         self.v_cache = [d.alloc(max_len * kv_dim) for _ in range(c.num_hidden_layers)]
         self.max_len = max_len
+        self.in8 = ()  # 8-bit weights: the inputs of the contractions
+        if model.q8:
+            self.xq, self.attq, self.gateq = self.in8 = [d.q8(BATCH, w) for w in (c.hidden_size, q_dim,
+                                                                                  c.intermediate_size)]
+            self.tail, self.tail_add = d.alloc(BATCH * c.hidden_size), d.alloc(BATCH * c.hidden_size)
+        self.scorers = {}  # OpModel.score: LogProbs by number of alternatives
+        self.all_logits = None  # ... and the logits of a batch
 
     def batch(self, device, n: int):
         if n > BATCH:
             raise ValueError(f"a batch of {n} tokens is more than {BATCH}")
         for buf, w in zip((self.x, self.xb, self.q, self.k, self.v, self.att, self.gate, self.up), self.widths):
             device.resize(buf, n * w)
+        for q in self.in8:
+            device.resize_q8(q, n)
 
 
 class OpModel:
-    """Model<D> (model/model.rs:11-149) driving `device` one trait call at a time."""
+    """Model<D> (model/model.rs:11-149) driving `device` one trait call at a time.
 
-    def __init__(self, config: Config, device, weights: dict):
-        self.config, self.device, self.w = config, device, weights
+    With q8=True the contractions run over 8-bit weights (a scale per output
+    channel, made from the checkpoint's bf16 at load time) and 8-bit inputs (a
+    scale per token): half the weights' bytes, and one plane of activations
+    instead of three. Norms, RoPE, attention and the residual stream stay f32."""
+
+    def __init__(self, config: Config, device, weights: dict, q8: bool = False):
+        self.config, self.device, self.w, self.q8 = config, device, weights, bool(q8)
+        if q8:
+            self.w = {k: device.quantize_weight(t) if k.endswith("_proj.weight") else t for k, t in weights.items()}
+            self.w["lm_head.weight"] = device.quantize_weight(
+                weights.get("lm_head.weight", weights["model.embed_tokens.weight"]))
 
     @classmethod
-    def load(cls, path: str, device) -> "OpModel":
+    def load(cls, path: str, device, q8: bool = False) -> "OpModel":
         c = Config.load(os.path.join(path, "config.json"))
-        return cls(c, device, load_weights(device, c, Weights.open(os.path.join(path, "model.safetensors"))))
+        return cls(c, device, load_weights(device, c, Weights.open(os.path.join(path, "model.safetensors"))), q8)
 
     def state(self, max_len: int, table=None) -> OpState:
         return OpState(self, max_len, table)
 
-    def forward(self, state: OpState, tokens, pos: int) -> np.ndarray:
-        tokens = list(tokens)
+    def _batches(self, state: OpState, tokens, pos: int):
+        """Runs the layers on up to BATCH tokens at a time; yields (first, n)
+        after each, the residual stream of those n tokens in state.x (and, with
+        8-bit weights, its last addend in state.xb)."""
         if not tokens:
             raise ValueError("no tokens to run")
         if pos + len(tokens) > state.max_len:
             raise ValueError("tokens past the end of the cache")
-        logits = None
         for i in range(0, len(tokens), BATCH):
-            logits = self._forward_batch(state, tokens[i:i + BATCH], pos + i)
-        return logits
+            part = tokens[i:i + BATCH]
+            self._layers(state, part, pos + i)
+            yield i, len(part)
 
-    def _forward_batch(self, s: OpState, tokens, pos: int) -> np.ndarray:
+    def forward(self, state: OpState, tokens, pos: int) -> np.ndarray:
+        for _, n in self._batches(state, list(tokens), pos):
+            self._head(state, n - 1, 1, state.logits)
+        return self.device.read(state.logits)
+
+    def score(self, state: OpState, tokens, pos: int, top: int = 0):
+        """Runs `tokens`, the first at `pos`, as `forward` does, and returns what
+        the model gives each of tokens[1:] where it stands: (logprob [n - 1],
+        entropy [n - 1], top_ids [n - 1, top], top_logprobs [n - 1, top])."""
+        tokens, d, vocab = list(tokens), self.device, self.config.vocab_size
+        if top not in state.scorers:
+            state.scorers[top] = LogProbs(d, BATCH, vocab, top)
+        if state.all_logits is None:
+            state.all_logits = d.alloc(BATCH * vocab)
+        parts = []
+        for i, n in self._batches(state, tokens, pos):
+            given = tokens[i + 1:i + n + 1]  # none for the last token
+            d.resize(state.all_logits, len(given) * vocab)
+            if given:
+                self._head(state, 0, len(given), state.all_logits)
+            parts.append(state.scorers[top].score(state.all_logits, given))
+        return tuple(np.concatenate(p) for p in zip(*parts))
+
+    def _layers(self, s: OpState, tokens, pos: int) -> None:
         c, d, w = self.config, self.device, self.w
         n, eps, hd = len(tokens), c.rms_norm_eps, c.head_dim()
         kv_dim = c.num_key_value_heads * hd
         s.batch(d, n)
         d.embed(s.x, w["model.embed_tokens.weight"], tokens)
+        added = None  # 8-bit weights: what the next norm adds to the residual stream first
         for i in range(c.num_hidden_layers):
             p = f"model.layers.{i}"
-            d.copy(s.xb, 0, s.x, 0, n * c.hidden_size)
-            d.rmsnorm(s.xb, w[f"{p}.input_layernorm.weight"], eps)
-            d.matmul(s.q, w[f"{p}.self_attn.q_proj.weight"], s.xb)
-            d.matmul(s.k, w[f"{p}.self_attn.k_proj.weight"], s.xb)
-            d.matmul(s.v, w[f"{p}.self_attn.v_proj.weight"], s.xb)
+            if self.q8:
+                d.add_rmsnorm_q8(s.xq, s.x, added, w[f"{p}.input_layernorm.weight"], eps)
+                for out, name in ((s.q, "q"), (s.k, "k"), (s.v, "v")):
+                    d.matmul_q8(out, w[f"{p}.self_attn.{name}_proj.weight"], s.xq)
+            else:
+                d.copy(s.xb, 0, s.x, 0, n * c.hidden_size)
+                d.rmsnorm(s.xb, w[f"{p}.input_layernorm.weight"], eps)
+                d.matmul(s.q, w[f"{p}.self_attn.q_proj.weight"], s.xb)
+                d.matmul(s.k, w[f"{p}.self_attn.k_proj.weight"], s.xb)
+                d.matmul(s.v, w[f"{p}.self_attn.v_proj.weight"], s.xb)
             if f"{p}.self_attn.q_norm.weight" in w:
                 d.rmsnorm(s.q, w[f"{p}.self_attn.q_norm.weight"], eps)
             if f"{p}.self_attn.k_norm.weight" in w:
@@ -223,6 +272,17 @@ class OpModel:
             d.copy(s.v_cache[i], pos * kv_dim, s.v, 0, n * kv_dim)
             d.attention(s.att, s.q, s.k_cache[i], s.v_cache[i], pos, c.num_attention_heads, hd,
                         c.num_key_value_heads)
+            if self.q8:
+                d.quantize(s.attq, s.att)
+                d.matmul_q8(s.xb, w[f"{p}.self_attn.o_proj.weight"], s.attq)
+                d.add_rmsnorm_q8(s.xq, s.x, s.xb, w[f"{p}.post_attention_layernorm.weight"], eps)
+                d.matmul_q8(s.gate, w[f"{p}.mlp.gate_proj.weight"], s.xq)
+                d.matmul_q8(s.up, w[f"{p}.mlp.up_proj.weight"], s.xq)
+                d.silu_mul(s.gate, s.up)
+                d.quantize(s.gateq, s.gate)
+                d.matmul_q8(s.xb, w[f"{p}.mlp.down_proj.weight"], s.gateq)
+                added = s.xb
+                continue
             d.matmul(s.xb, w[f"{p}.self_attn.o_proj.weight"], s.att)
             d.add(s.x, s.xb)
             d.copy(s.xb, 0, s.x, 0, n * c.hidden_size)
@@ -232,11 +292,24 @@ class OpModel:
             d.silu_mul(s.gate, s.up)
             d.matmul(s.xb, w[f"{p}.mlp.down_proj.weight"], s.gate)
             d.add(s.x, s.xb)
-        d.resize(s.xb, c.hidden_size)
-        d.copy(s.xb, 0, s.x, (n - 1) * c.hidden_size, c.hidden_size)
-        d.rmsnorm(s.xb, w["model.norm.weight"], eps)
-        d.matmul(s.logits, w.get("lm_head.weight", w["model.embed_tokens.weight"]), s.xb)
-        return d.read(s.logits)
+
+    def _head(self, s: OpState, first: int, n: int, logits) -> None:
+        """The final norm and lm_head of rows first .. first + n - 1 of the batch."""
+        c, d, w = self.config, self.device, self.w
+        norm, h = w["model.norm.weight"], c.hidden_size
+        if self.q8:
+            d.resize(s.tail, n * h)
+            d.resize(s.tail_add, n * h)
+            d.copy(s.tail, 0, s.x, first * h, n * h)
+            d.copy(s.tail_add, 0, s.xb, first * h, n * h)
+            d.resize_q8(s.xq, n)
+            d.add_rmsnorm_q8(s.xq, s.tail, s.tail_add, norm, c.rms_norm_eps)
+            d.matmul_q8(logits, w["lm_head.weight"], s.xq)
+            return
+        d.resize(s.xb, n * h)
+        d.copy(s.xb, 0, s.x, first * h, n * h)
+        d.rmsnorm(s.xb, norm, c.rms_norm_eps)
+        d.matmul(logits, w.get("lm_head.weight", w["model.embed_tokens.weight"]), s.xb)
 
 
 # ---- the fused fast path -------------------------------------------------------
@@ -522,6 +595,67 @@ class DeviceSampler:
     def close(self) -> None:
         if getattr(self, "_h", None) and not sys.is_finalizing():
             _lib.lib().tb200_sampler_free(self._h)
+        self._h = None
+
+    __del__ = close
+
+
+class LogProbs:
+    """Log probabilities of given tokens, with each row's entropy and its `top`
+    most likely alternatives, from logits in a device buffer (tb200_score). The
+    results of the last call stay on the device as `logprob` and `entropy`
+    ([rows] f32), `top_ids` ([rows, top] int32) and `top_logprobs` (f32)."""
+
+    def __init__(self, dev: B200, rows: int, vocab: int, top: int = 0):
+        self._dev, self.rows, self.vocab, self.top = dev, int(rows), int(vocab), int(top)
+        h = ctypes.c_void_p()
+        call("tb200_scorer_new", dev._h, self.rows, self.vocab, self.top, ctypes.byref(h))
+        self._h = h.value
+
+    def _array(self, which, shape, typestr):
+        p = [ctypes.c_void_p() for _ in range(4)]
+        call("tb200_scorer_data", self._h, *[ctypes.byref(x) for x in p])
+        return DeviceArray(self, self._dev, p[which].value, shape, typestr)
+
+    logprob = property(lambda self: self._array(0, (self.rows,), "<f4"))
+    entropy = property(lambda self: self._array(1, (self.rows,), "<f4"))
+    top_ids = property(lambda self: self._array(2, (self.rows, self.top), "<i4"))
+    top_logprobs = property(lambda self: self._array(3, (self.rows, self.top), "<f4"))
+
+    @staticmethod
+    def _tokens(tokens):
+        """(pointer, n, what keeps it alive) of ids on the device (anything with
+        the CUDA array interface, 32-bit integers) or on the host."""
+        a = getattr(tokens, "__cuda_array_interface__", None)
+        if a is None:
+            t = np.ascontiguousarray(tokens, dtype=np.uint32).reshape(-1)
+            return t.ctypes.data, t.size, t
+        n = int(np.prod(a["shape"]))
+        if a["typestr"] not in ("<i4", "<u4") or (a.get("strides") and n > 1 and (
+                len(a["shape"]) != 1 or a["strides"][0] != 4)):
+            raise ValueError("token ids on the device must be contiguous 32-bit integers")
+        return a["data"][0], n, tokens
+
+    def enqueue(self, logits, tokens) -> None:
+        """Row i of `logits` ([n, vocab] f32 in a device Buffer) is scored at
+        tokens[i]; the results stay on the device and nothing waits. Token ids
+        on the device are read in order with the device's stream."""
+        ptr, n, _ = self._tokens(tokens)
+        call("tb200_score_enqueue", self._h, logits._h, ctypes.cast(ptr, _lib.U32P), n)
+
+    def score(self, logits, tokens):
+        """`enqueue`, then (logprob [n], entropy [n], top_ids [n, top],
+        top_logprobs [n, top]) on the host."""
+        ptr, n, _ = self._tokens(tokens)
+        lp, ent = np.empty(n, dtype=np.float32), np.empty(n, dtype=np.float32)
+        ids, tlp = np.empty((n, self.top), dtype=np.uint32), np.empty((n, self.top), dtype=np.float32)
+        call("tb200_score", self._h, logits._h, ctypes.cast(ptr, _lib.U32P), n, lp.ctypes.data_as(_lib.F32P),
+             ent.ctypes.data_as(_lib.F32P), ids.ctypes.data_as(_lib.U32P), tlp.ctypes.data_as(_lib.F32P))
+        return lp, ent, ids, tlp
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) and self._dev._h and not sys.is_finalizing():
+            _lib.lib().tb200_scorer_free(self._h)
         self._h = None
 
     __del__ = close
