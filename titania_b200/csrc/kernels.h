@@ -243,6 +243,8 @@ void launch_gemm(cudaStream_t s, const GemmPlan& p, int epilogue, const CUtensor
 // ---- many-token forward around the contractions (batch.cu) ------------------
 
 cudaError_t init_batch_kernels();
+// q8_gemm.cu: raises the shared-memory limits of the 8-bit product's kernels.
+cudaError_t init_q8_kernels();
 // Query heads per kv head that the batched attention kernels handle.
 bool batch_group_supported(int group);
 // Cache positions per chunk of the decode attention (launch_attn_rows).

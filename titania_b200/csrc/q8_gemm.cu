@@ -4,7 +4,33 @@
 //
 // The sum is exact in 32-bit integers (|q| <= 128 and at most 131071 columns),
 // so its order is free; the two f32 roundings of the scales' product and the
-// final product follow it.
+// final product follow it. Every variant below gives the same bits.
+//
+// k_matvec_q8 (few tokens): a warp per channel, dp4a on CUDA cores.
+// k_gemm_q8 (more): tcgen05.mma kind::i8, s8 x s8 into s32 accumulators in
+// tensor memory. Tokens are the rows of the accumulator (M = 128 a CTA),
+// channels its columns (N, a multiple of 16 chosen per call). A lane then
+// holds runs of one output row, and N can be fitted to the number of
+// channels so that the tiles come out even over the SMs.
+//   warp 0     producer: per 128 columns of K, a box of up to 128 token rows
+//              and one of N channel rows (128-byte swizzle) into a ring;
+//   warp 1     one lane issues the MMAs (K = 32 each), commits each stage back
+//              to the producer and each tile to the epilogue;
+//   warps 2-5  epilogue: tcgen05.ld, scales, stores; two accumulators let it
+//              run behind the next tile's MMAs.
+// Persistent CTAs walk the tiles, token tiles innermost, so that a channel
+// tile comes from memory once. Only the token rows that exist are loaded: the
+// MMA reads whatever shared memory holds in the place of the others, and the
+// accumulator rows that this makes are never read.
+//
+// Every mbarrier wait is bounded (kWaitCycles); on expiry the kernel leaves
+// TB200_ERR_TIMEOUT in the device's async error word, lets what it issued
+// drain, frees its tensor memory and returns. Every CTA takes more than half
+// of an SM's shared memory, so no two share an SM and the allocation of
+// tensor memory never waits.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <string>
 
@@ -12,7 +38,6 @@
 
 namespace tb {
 namespace {
-
 constexpr size_t kMaxCols = 131071;  // 128 * 128 * 131071 < 2^31
 
 // One warp per channel and up to 4 tokens.
@@ -45,7 +70,318 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
   }
 }
 
+
+// ---- tensor cores ------------------------------------------------------------
+
+constexpr int kTileM = 128;              // token rows per CTA
+constexpr int kMaxN = 256;               // channels per tile
+constexpr int kKB = 128;                 // K per stage: one 128-byte swizzle row
+constexpr int kQThreads = 192;
+constexpr int kQTmemCols = 512;          // two accumulators of up to 256 columns
+constexpr int kQMaxStages = 24;
+constexpr size_t kQMinSmem = 116 * 1024;  // more than half of an SM's 228 KB
+constexpr size_t kQMaxSmem = 226 * 1024;
+
+struct QGemmArgs {
+  const float* sw;
+  const float* sx;
+  float* out;
+  int T, M, K;       // tokens, channels, columns
+  int n;             // channels per tile
+  int xrows;         // token rows per tile that are loaded (a multiple of 8, at most 128)
+  int stages, mtiles, ntiles;
+  int vec;           // floats per store that the output rows' alignment allows: 8, 4 or 1
+  int* err;
+};
+
+// Shared memory after the ring: barriers full[s], empty[s], tfull[2], tempty[2],
+// mdone, then the address of the tensor memory and the epilogue's scales.
+struct QTail {
+  uint64_t full[kQMaxStages], empty[kQMaxStages], tfull[2], tempty[2], mdone;
+  uint32_t tmem;
+  int ok[4];
+  alignas(16) float sw[2][kMaxN];
+};
+
+__host__ __device__ constexpr size_t q_stage_bytes(int n, int xrows) { return size_t(n + xrows) * kKB; }
+// The last stage's MMA reads 128 token rows whatever xrows is.
+__host__ __device__ constexpr size_t q_ring_bytes(int n, int xrows, int stages) {
+  return stages * q_stage_bytes(n, xrows) + size_t(kTileM - xrows) * kKB;
+}
+
+__device__ __forceinline__ void q_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void q_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Shared-memory matrix descriptor of a K-major operand in rows of 128 bytes,
+// 128-byte swizzle, groups of 8 rows 1024 bytes apart: start address >> 4
+// [0,14), leading byte offset >> 4 [16,30) (unused here, 1), stride byte
+// offset >> 4 [32,46), version 1 [46,48), layout 2 = 128-byte swizzle [61,64).
+__device__ __forceinline__ uint64_t q_desc(uint32_t saddr) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// Instruction descriptor, kind::i8: s32 accumulator [4,6) = 2, A and B signed
+// ([7,10) = 1, [10,13) = 1), both K-major, N >> 3 at [17,23), M >> 4 at [24,29).
+__device__ __forceinline__ uint32_t q_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+__device__ __forceinline__ void q_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void q_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 16 consecutive 32-bit columns of this warp's 32 lanes.
+__device__ __forceinline__ void q_tmem_ld16(uint32_t addr, int (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Eight floats to a 32-byte aligned address in one store (a whole sector).
+__device__ __forceinline__ void st8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+__global__ void __launch_bounds__(kQThreads, 1)
+    k_gemm_q8(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, QGemmArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles: 1024-byte alignment
+  const int stages = a.stages, n = a.n;
+  const uint32_t stage_bytes = uint32_t(q_stage_bytes(n, a.xrows));
+  QTail& tl = *reinterpret_cast<QTail*>(sm + q_ring_bytes(n, a.xrows, stages));
+  auto sB = [&](int s) { return sm + size_t(s) * stage_bytes; };
+  auto sA = [&](int s) { return sm + size_t(s) * stage_bytes + size_t(n) * kKB; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nkb = (a.K + kKB - 1) / kKB;
+  const int tiles = a.mtiles * a.ntiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; s++) {
+      mbar_init(&tl.full[s], 1);
+      mbar_init(&tl.empty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&tl.tfull[b], 1);
+      mbar_init(&tl.tempty[b], 4);  // one arrival per epilogue warp
+    }
+    mbar_init(&tl.mdone, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tl.tmem)),
+                 "r"(kQTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  q_fence_before();
+  __syncthreads();
+  q_fence_after();
+  const uint32_t tmem = tl.tmem;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
+      int i = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
+        for (int k = 0; k < nkb; k++, i++) {
+          const int s = i % stages;
+          if (!mbar_wait(&tl.empty[s], ((i / stages) & 1) ^ 1, a.err)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&tl.full[s], stage_bytes);
+          tma_load_2d(sB(s), &tw, k * kKB, n0, &tl.full[s], pol_w);
+          tma_load_2d(sA(s), &tx, k * kKB, m0, &tl.full[s], pol_x);
+        }
+      }
+      // Every issued copy has landed before the CTA can exit.
+      for (int j = i - 1; j >= 0 && j >= i - stages; j--) mbar_wait(&tl.full[j % stages], (j / stages) & 1, nullptr);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = q_idesc(kTileM, n);
+      int i = 0, ti = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ti++) {
+        const int b = ti & 1;
+        // The epilogue has drained this accumulator's previous tile.
+        if (!mbar_wait(&tl.tempty[b], ((ti >> 1) - 1) & 1, a.err)) break;
+        q_fence_after();
+        const uint32_t acc = tmem + uint32_t(b * kMaxN);
+        for (int k = 0; k < nkb; k++, i++) {
+          const int s = i % stages;
+          if (!mbar_wait(&tl.full[s], (i / stages) & 1, a.err)) {
+            ok = false;
+            break;
+          }
+          q_fence_after();
+          const uint32_t a0 = smem_u32(sA(s)), b0 = smem_u32(sB(s));
+#pragma unroll
+          for (int kk = 0; kk < kKB / 32; kk++)
+            q_mma(acc, q_desc(a0 + 32 * kk), q_desc(b0 + 32 * kk), idesc, (k > 0 || kk > 0) ? 1u : 0u);
+          q_commit(&tl.empty[s]);
+        }
+        if (ok) q_commit(&tl.tfull[b]);
+      }
+      // Tensor memory is freed below only after every MMA has completed.
+      q_commit(&tl.mdone);
+      mbar_wait(&tl.mdone, 0, nullptr);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;  // the 32 accumulator lanes this warp can read
+    const int e = int(threadIdx.x) - 64;
+    int ti = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ti++) {
+      const int b = ti & 1;
+      const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
+      const int cols = min(n, a.M - n0);
+      for (int j = e; j < n; j += 128) tl.sw[b][j] = j < cols ? a.sw[n0 + j] : 0.f;
+      const int t = m0 + 32 * q + lane;
+      const float sx = t < a.T ? a.sx[t] : 0.f;
+      // The four warps take the same way out: a verdict is shared. The
+      // barriers also put tl.sw in place.
+      const bool mine = __all_sync(0xffffffffu, mbar_wait(&tl.tfull[b], (ti >> 1) & 1, a.err));
+      if (lane == 0) tl.ok[q] = mine;
+      named_sync(1, 128);
+      const bool ok = tl.ok[0] && tl.ok[1] && tl.ok[2] && tl.ok[3];
+      named_sync(1, 128);
+      if (!ok) break;
+      q_fence_after();
+      if (m0 + 32 * q < a.T) {  // warp-uniform: some of this warp's tokens exist
+        const uint32_t taddr = tmem + uint32_t(b * kMaxN) + (uint32_t(32 * q) << 16);
+        float* row = a.out + size_t(t) * a.M + n0;
+        for (int c = 0; c < cols; c += 16) {
+          int acc[16];
+          q_tmem_ld16(taddr + c, acc);
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++) v[j] = __fmul_rn(__int2float_rn(acc[j]), __fmul_rn(tl.sw[b][c + j], sx));
+          if (t >= a.T) {
+            // no such token
+          } else if (a.vec == 8 && c + 16 <= cols) {
+            st8(row + c, v);
+            st8(row + c + 8, v + 8);
+          } else if (a.vec >= 4 && c + 16 <= cols) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(row + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+              if (c + j < cols) row[c + j] = v[j];
+          }
+          __syncwarp();  // the next tcgen05.ld is the whole warp's
+        }
+      }
+      q_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tl.tempty[b]);
+    }
+  }
+  q_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    q_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kQTmemCols) : "memory");
+  }
+}
+
+// Tensor map of 8-bit rows in boxes of 128 columns by box_rows rows.
+int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult r{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  if (!encode) return rt::fail(TB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {cuuint64_t(q->ld), cuuint64_t(q->cap)};
+  cuuint64_t strides[1] = {cuuint64_t(q->ld)};
+  cuuint32_t box[2] = {cuuint32_t(kKB), cuuint32_t(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q->values, dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return rt::fail(TB200_ERR_CUDA, "matmul_q8: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+  return TB200_OK;
+}
+
+// Channels per tile: the multiple of 16 with which the CTA that has most to do
+// has least, a tile's fixed cost (filling the ring, the last tile's epilogue)
+// counted as 24 channels.
+int plan_n(int M, int mtiles, int sms) {
+  int best = 0;
+  long long least = 0;
+  for (int n = 16; n <= kMaxN; n += 16) {
+    const long long tiles = (long long)mtiles * ((M + n - 1) / n);
+    const long long cost = (tiles + sms - 1) / sms * (n + 24);
+    if (!best || cost <= least) best = n, least = cost;
+  }
+  return best;
+}
+
+int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
+  QGemmArgs a{};
+  a.sw = w->scales;
+  a.sx = x->scales;
+  a.out = out;
+  a.T = int(x->rows);
+  a.M = int(w->rows);
+  a.K = int(w->cols);
+  a.err = d->async_err_dev;
+  a.mtiles = (a.T + kTileM - 1) / kTileM;
+  a.n = plan_n(a.M, a.mtiles, d->sms);
+  a.ntiles = (a.M + a.n - 1) / a.n;
+  a.xrows = std::min(kTileM, (a.T + 7) / 8 * 8);
+  const size_t fixed = size_t(kTileM - a.xrows) * kKB + sizeof(QTail) + 1024;
+  a.stages = int(std::min<size_t>(kQMaxStages, (kQMaxSmem - fixed) / q_stage_bytes(a.n, a.xrows)));
+  const uintptr_t al = reinterpret_cast<uintptr_t>(out) | (uintptr_t(a.M) * 4);
+  a.vec = al % 32 == 0 ? 8 : al % 16 == 0 ? 4 : 1;
+  CUtensorMap tw, tx;
+  if (int rc = encode_tmap_q8(&tw, w, a.n)) return rc;
+  if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
+  const size_t smem =
+      std::max(kQMinSmem, q_ring_bytes(a.n, a.xrows, a.stages) + sizeof(QTail) + 1024);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(std::min<long long>((long long)a.mtiles * a.ntiles, d->sms)));
+  cfg.blockDim = dim3(kQThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = d->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, k_gemm_q8, tw, tx, a);
+  return rt::launched("matmul_q8");
+}
+
 }  // namespace
+
+cudaError_t init_q8_kernels() {
+  return cudaFuncSetAttribute(k_gemm_q8, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
+}
+
 }  // namespace tb
 
 extern "C" {
@@ -59,6 +395,7 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   ARG_CHECK(out->len == x->rows * w->rows, "matmul_q8: output holds " + std::to_string(out->len) + ", expected " +
                                                std::to_string(x->rows * w->rows));
   if (!x->rows || !w->rows) return TB200_OK;
+  if (x->rows > 4) return tb::gemm_q8(d, out->ptr, w, x);
   const dim3 grid(unsigned((w->rows + 7) / 8), unsigned((x->rows + 3) / 4));
   tb::k_matvec_q8<<<grid, 256, 0, d->stream>>>(out->ptr, w->values, w->scales, int(w->rows), x->values, x->scales,
                                                int(x->rows), int(w->ld), int(x->ld));

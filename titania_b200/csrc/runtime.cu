@@ -156,6 +156,7 @@ int tb200_device_open(int ordinal, tb200_device** out) {
   cudaError_t e = tb::init_fused_kernels(int(prop.sharedMemPerBlockOptin));
   if (e == cudaSuccess) e = tb::init_gemm_kernels();
   if (e == cudaSuccess) e = tb::init_batch_kernels();
+  if (e == cudaSuccess) e = tb::init_q8_kernels();
   if (e != cudaSuccess) return fail(TB200_ERR_CUDA, std::string("kernel setup: ") + cudaGetErrorString(e));
   auto* d = new tb200_device;
   d->ordinal = ordinal;
