@@ -485,16 +485,7 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.chunks = tb::score_chunks(s->dev, n, a.max_blocks);
   a.chunk_blocks = (a.max_blocks + a.chunks - 1) / a.chunks;
   a.chunks = (a.max_blocks + a.chunk_blocks - 1) / a.chunk_blocks;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(n * a.chunks));
-  cfg.blockDim = dim3(tb::kScoreThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, tb::k_score, a);
+  tb::launch_pdl(tb::k_score, dim3(unsigned(n * a.chunks)), dim3(tb::kScoreThreads), 0, st, a);
   return rt::launched("score");
 }
 

@@ -45,6 +45,8 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
                                                    const float* __restrict__ sw, int channels,
                                                    const int8_t* __restrict__ x, const float* __restrict__ sx,
                                                    int tokens, int ldw, int ldx) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x * 8 + warp, t0 = blockIdx.y * 4;
   if (c >= channels) return;
@@ -362,17 +364,8 @@ int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
   const size_t smem =
       std::max(kQMinSmem, q_ring_bytes(a.n, a.xrows, a.stages) + sizeof(QTail) + 1024);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(std::min<long long>((long long)a.mtiles * a.ntiles, d->sms)));
-  cfg.blockDim = dim3(kQThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = d->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, k_gemm_q8, tw, tx, a);
+  const unsigned grid = unsigned(std::min<long long>((long long)a.mtiles * a.ntiles, d->sms));
+  launch_pdl(k_gemm_q8, dim3(grid), dim3(kQThreads), smem, d->stream, tw, tx, a);
   return rt::launched("matmul_q8");
 }
 
@@ -397,8 +390,8 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   if (!x->rows || !w->rows) return TB200_OK;
   if (x->rows > 4) return tb::gemm_q8(d, out->ptr, w, x);
   const dim3 grid(unsigned((w->rows + 7) / 8), unsigned((x->rows + 3) / 4));
-  tb::k_matvec_q8<<<grid, 256, 0, d->stream>>>(out->ptr, w->values, w->scales, int(w->rows), x->values, x->scales,
-                                               int(x->rows), int(w->ld), int(x->ld));
+  tb::launch_pdl(tb::k_matvec_q8, grid, dim3(256), 0, d->stream, out->ptr, w->values, w->scales, int(w->rows),
+                 x->values, x->scales, int(x->rows), int(w->ld), int(x->ld));
   return rt::launched("matmul_q8");
 }
 
