@@ -11,16 +11,20 @@
 // Both terms of the entropy are positive and log1p keeps S's relative error,
 // so neither loses digits when one token has almost all of the probability.
 //
-// One launch, one pass over the logits, bound by reading them. A row is cut
-// into chunks, a CTA each (few rows) or several rows' chunks fill the GPU
-// (many). A warp takes 128 logits (a block) at a time: their largest, one
-// redux, is both the running maximum that the sums refer to, so that rescaling
-// is a rare warp-uniform branch, and the block's entry in a table of 1/128 of
-// the logits' size. The last CTA of a row joins the chunks' sums and finds
-// the alternatives: the k largest logits lie in the k blocks with the largest
-// maxima (each of those has an element at least as large as any element of
-// another block), so only those blocks are read again.
+// One launch, one pass over the logits, bound by reading them. The rows' steps
+// of 512 logits, one after another, are dealt out to the CTAs in equal runs
+// (whatever the number of rows, no SM waits for another's last row); a CTA's
+// part of a row is a piece. A warp takes a step at a time, as four blocks of
+// 128: their largest, a redux each, are both the running maximum that the sums
+// refer to, so that rescaling is a rare warp-uniform branch, and the blocks'
+// entries in a table of 1/128 of the logits' size. Per logit that leaves five
+// instructions for the sums and one for the maximum; at ten it was bound by
+// them (1111 x 151936: 142 us, against 105 us for the bytes). The CTA that finishes a row's last piece joins the pieces'
+// sums, in their order, and finds the alternatives: the k largest logits lie in
+// the k blocks with the largest maxima (each of those has an element at least as
+// large as any element of another block), so only those blocks are read again.
 #include <algorithm>
+#include <climits>
 #include <string>
 
 #include "runtime.h"
@@ -32,9 +36,10 @@ struct tb200_scorer {
   float *logprob = nullptr, *entropy = nullptr, *top_logprobs = nullptr;
   uint32_t* top_ids = nullptr;
   uint32_t* tokens = nullptr;   // [rows] ids given in host memory
-  float4* part = nullptr;       // sums of the chunks
-  int* block_max = nullptr;     // [rows][blocks], when there are alternatives
+  float4* part = nullptr;       // sums of the pieces
+  int* block_max = nullptr;     // [rows][a row's blocks], when there are alternatives
   unsigned* ticket = nullptr;   // [rows], zero between launches
+  int ctas = 0;                 // that the GPU runs at once
 };
 
 namespace tb {
@@ -43,10 +48,11 @@ namespace {
 constexpr int kScoreThreads = 256;
 constexpr int kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreMaxTop = 64;
-constexpr int kBlock = 128;        // logits per warp step and table entry
-constexpr int kUnroll = 4;         // blocks a warp has in flight
-constexpr int kCand = 1024;        // candidates ranked in shared memory
-constexpr int kOwn = 8;            // table entries a thread keeps in registers
+constexpr int kBlock = 128;        // logits per table entry
+constexpr int kStep = 4;           // blocks a warp takes at a time
+constexpr int kCand = 2048;        // candidates held in shared memory
+constexpr int kOwn = 8;            // table entries or candidates a thread keeps in registers
+static_assert(kCand == kOwn * kScoreThreads, "a thread's candidates fit its registers");
 constexpr int kNegInf = int(0xFF800000u ^ 0x7FFFFFFFu);  // order(-inf)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -117,58 +123,111 @@ struct Row {
   }
 };
 
-// Adds a block to the warp's set (a.m is the warp's, a.s and a.t each lane's
-// share). bm: the block's largest in order.
-__device__ __forceinline__ void add_block(Soft& a, float4 v, int bm, int lane) {
-  float x[4] = {v.x, v.y, v.z, v.w};
-  if (bm <= kNegInf) {  // nothing but excluded tokens; a NaN below them counts
-    if (isnan(x[0]) || isnan(x[1]) || isnan(x[2]) || isnan(x[3])) a.s = __int_as_float(0x7FC00000);
-    return;
+// A warp's set while it grows: m is the warp's, s and t each lane's shares of
+// the sums, taken at c = f32(m log2 e) in the place of m log2 e, which saves an
+// instruction a logit: what that leaves out (lo) is put right in settled().
+struct Running {
+  float m, c, lo, s, t;
+  int order;  // of m
+  __device__ __forceinline__ Running() : m(-INFINITY), c(0.f), lo(0.f), s(0.f), t(0.f), order(kNegInf) {}
+  __device__ __forceinline__ Soft settled() const {
+    const float f = ex2(-lo);
+    return Soft{m, s * f, fmaf(lo, s, t) * f};
   }
-  float skip[4] = {0.f, 0.f, 0.f, 0.f};
-  if (bm > order(a.m)) {  // warp-uniform: a new maximum
-    const float m = unorder(bm);
-    // Lane 0 carries the old maximum's own term; every lane its share of the others'.
-    const float d = (m - a.m) * kLog2e, e = ex2(-d);
-    if (a.m == -INFINITY) {
-      // nothing yet (or a NaN, which stays)
-    } else if (e == 0.0f) {
-      a.s *= 0.0f;
-      a.t = 0.0f;
-    } else {
-      const float s = lane == 0 ? fmaf(e, a.s, e) : e * a.s;
-      a.t = fmaf(e, a.t, d * s);
-      a.s = s;
+  // Refers the sums to a larger maximum; lane 0 takes the old one's own term.
+  __device__ __forceinline__ void raise(int bm, int lane) {
+    const Soft old = settled();
+    const float nm = unorder(bm);
+    if (order > kNegInf) {
+      const float d = (nm - old.m) * kLog2e, e = ex2(-d);
+      if (e == 0.0f) {
+        s = old.s * 0.0f;  // a NaN stays
+        t = 0.0f;
+      } else {
+        s = lane == 0 ? fmaf(e, old.s, e) : e * old.s;
+        t = fmaf(e, old.t, d * s);
+      }
     }
-    a.m = m;
-    // The maximum itself stays out of the sums: its first place in the block.
-    const int mine = order(x[0]) == bm ? 0 : order(x[1]) == bm ? 1 : order(x[2]) == bm ? 2 : order(x[3]) == bm ? 3 : 4;
-    const unsigned who = __ballot_sync(0xffffffffu, mine < 4);
+    m = nm;
+    order = bm;
+    c = m * kLog2e;
+    lo = huge() ? 0.f : fmaf(m, kLog2e, -c);
+  }
+  // Whether m log2 e may be past f32's range.
+  __device__ __forceinline__ bool huge() const { return fabsf(m) > 1e38f; }
+  // A logit's share of the sums. Far below the maximum (or excluded) it adds 0, not 0 * -inf.
+  template <bool HUGE>
+  __device__ __forceinline__ void add(float x) {
+    const float d = fmaxf(HUGE ? (x - m) * kLog2e : fmaf(x, kLog2e, -c), -200.0f);
+    const float e = ex2(d);
+    s += e;
+    t = fmaf(-d, e, t);
+  }
+};
+
+// Four blocks: their largest in order go to bm, their sums to a. `real(u, j)`
+// is whether value j of block u is the row's (`whole`: all are).
+template <class Real>
+__device__ __forceinline__ void add_step(Running& a, float4 (&v)[kStep], int (&bm)[kStep], int lane, bool whole,
+                                         Real real) {
+  float x[kStep][4];
+  float m[kStep], least = INFINITY;
+#pragma unroll
+  for (int u = 0; u < kStep; u++) {
+    x[u][0] = v[u].x, x[u][1] = v[u].y, x[u][2] = v[u].z, x[u][3] = v[u].w;
+    m[u] = x[u][0];
+#pragma unroll
+    for (int j = 1; j < 4; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[u]) : "f"(x[u][j]));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(least) : "f"(fabsf(m[u])));
+    bm[u] = order(m[u]);
+  }
+  // By integers where floats do not decide: NaNs, of which one sign is the
+  // highest in order and the other the lowest, zeros of both signs, and
+  // places behind the row's ends, which are lowest of all.
+  if (!whole || !(least > 0.0f)) {
+#pragma unroll
+    for (int u = 0; u < kStep; u++) {
+      bm[u] = INT_MIN;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (real(u, j)) bm[u] = max(bm[u], order(x[u][j]));
+        if (isnan(x[u][j])) a.s = x[u][j];
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < kStep; u++) bm[u] = __reduce_max_sync(0xffffffffu, bm[u]);
+  const int top = max(max(bm[0], bm[1]), max(bm[2], bm[3]));
+  if (top > a.order) {  // a new maximum, the same for the warp
+    a.raise(top, lane);
+    // It stays out of the sums itself: its first place in the step.
+    int mine = kStep * 4;
+#pragma unroll
+    for (int i = kStep * 4 - 1; i >= 0; i--)
+      if (order(x[i / 4][i % 4]) == top && real(i / 4, i % 4)) mine = i;
+    const unsigned who = __ballot_sync(0xffffffffu, mine < kStep * 4);
     if (lane == __ffs(who) - 1) {
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (j == mine) skip[j] = -INFINITY;
+      for (int i = 0; i < kStep * 4; i++)
+        if (i == mine) x[i / 4][i % 4] = -INFINITY;
     }
   }
-  float e[4], d[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    d[j] = (x[j] - a.m) * kLog2e + skip[j];
-    e[j] = ex2(d[j]);
-    d[j] = fmaxf(d[j], -200.0f);  // 0 * -inf has to be 0
+  if (a.order <= kNegInf) return;  // nothing but excluded tokens so far
+  if (a.huge()) {
+    for (int i = 0; i < kStep * 4; i++) a.add<true>(x[i / 4][i % 4]);
+    return;
   }
-  a.s += (e[0] + e[1]) + (e[2] + e[3]);
-  a.t -= fmaf(d[0], e[0], d[1] * e[1]) + fmaf(d[2], e[2], d[3] * e[3]);
+#pragma unroll
+  for (int i = 0; i < kStep * 4; i++) a.add<false>(x[i / 4][i % 4]);
 }
 
-__device__ __forceinline__ int max4(float4 v) { return max(max(order(v.x), order(v.y)), max(order(v.z), order(v.w))); }
-
 // A key with k <= #{keys >= it} <= most: bisection over 64-bit keys that no
-// two entries share. count(key) is called by all threads and is the same for
-// all; at least k keys exist.
+// two entries share, none above hi and at least k of them lo or above.
+// count(key) is called by all threads and is the same for all.
 template <class Count>
-__device__ __forceinline__ unsigned long long key_bound(int k, int most, Count count) {
-  unsigned long long lo = 0, hi = ~0ull;  // count(lo) >= k; count(hi + 1) < k
+__device__ __forceinline__ unsigned long long key_bound(int k, int most, unsigned long long lo, unsigned long long hi,
+                                                        Count count) {
   while (lo < hi) {
     const unsigned long long mid = lo + (hi - lo) / 2 + 1;
     const int c = count(mid);
@@ -187,10 +246,13 @@ struct ScoreArgs {
   const uint32_t* tokens;
   float *logprob, *entropy, *top_logprobs;
   uint32_t* top_ids;
-  float4* part;     // [rows][chunks]
-  int* block_max;   // [rows][max_blocks]
+  float4* part;     // piece of row r by CTA c: [r + c]
+  int* block_max;   // [rows][steps * kStep]
   unsigned* ticket;
-  int vocab, top, chunks, chunk_blocks, max_blocks;
+  int vocab, top;
+  int steps;        // of a row, whatever its alignment
+  long long total;  // steps of all rows
+  long long run;    // steps of a CTA
 };
 
 struct ScoreShared {
@@ -198,7 +260,7 @@ struct ScoreShared {
   int last, n_blocks, n_cand;
   int counts[2][kScoreWarps];
   unsigned long long cand[kCand];
-  int blocks[kScoreMaxTop + kScoreMaxTop / 2 + 4];
+  int blocks[kScoreMaxTop + kScoreMaxTop / 2 + 16];
 };
 
 // The sum of c over the CTA, on every thread. Calls take `turn` 0, 1, 0, ... in
@@ -220,17 +282,32 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
                              ScoreShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k = a.top;
+  // No key is above this one. (m's sign is not relied on where it is zero.)
+  const unsigned long long highest = m > 0.0f && !isnan(logz) ? order_key(order(m), 0) : ~0ull;
   int turn = 0;
   if (threadIdx.x == 0) sh.n_blocks = sh.n_cand = 0;
-  // The blocks with the largest maxima: k of them, or more where that ends the search sooner.
   unsigned long long own[kOwn];
+  // The blocks with the largest maxima: k of them, or more where that ends the search sooner.
 #pragma unroll
   for (int i = 0; i < kOwn; i++) {
     const int b = int(threadIdx.x) + i * kScoreThreads;
     own[i] = b < r.blocks ? order_key(__ldcg(block_max + b), uint32_t(b)) : 0ull;
   }
   const int kb = min(k, r.blocks);
-  const unsigned long long bound = key_bound(kb, kb + kb / 2 + 4, [&](unsigned long long key) {
+  // Where every thread has a block, the least of their largest has 256 >= k keys at or above it.
+  unsigned long long lo = 0;
+  if (r.blocks >= kScoreThreads) {
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; i++) mine = max(mine, unsigned(own[i] >> 32));
+    mine = __reduce_min_sync(0xffffffffu, mine);
+    if (lane == 0) sh.counts[1][warp] = int(mine);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kScoreWarps; w++) mine = min(mine, unsigned(sh.counts[1][w]));
+    lo = static_cast<unsigned long long>(mine) << 32;
+  }
+  unsigned long long bound = key_bound(kb, kb + kb / 2 + 16, lo, highest, [&](unsigned long long key) {
     int c = 0;
 #pragma unroll
     for (int i = 0; i < kOwn; i++) c += own[i] >= key;
@@ -261,10 +338,7 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
       }
     }
   };
-  // Candidates: the elements at least as large as the smallest of the picked
-  // maxima (k of these exist), or all elements where there are fewer blocks than k.
-  unsigned long long least = r.blocks < k ? 0ull : bound & 0xFFFFFFFF00000000ull;
-  for (int tries = 0; tries < 2; tries++) {
+  auto collect = [&](unsigned long long least) {
     each([&](unsigned long long key) {
       if (key >= least && key) {
         const int at = atomicAdd(&sh.n_cand, 1);
@@ -272,9 +346,13 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
       }
     });
     __syncthreads();
-    if (sh.n_cand <= kCand) break;
+  };
+  // Candidates: the elements at least as large as the smallest of the picked
+  // maxima (k of these exist), or all elements where there are fewer blocks than k.
+  collect(r.blocks < k ? 0ull : bound & 0xFFFFFFFF00000000ull);
+  if (sh.n_cand > kCand) {
     // More than there is room for (neighbours that are all large): a bound that leaves fewer.
-    least = key_bound(k, kCand, [&](unsigned long long key) {
+    bound = key_bound(k, kCand, 0ull, highest, [&](unsigned long long key) {
       int c = 0;
       each([&](unsigned long long x) { c += x >= key; });
       return cta_sum(c, turn, sh);
@@ -282,8 +360,31 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
     __syncthreads();
     if (threadIdx.x == 0) sh.n_cand = 0;
     __syncthreads();
+    collect(bound);
   }
-  const int n = sh.n_cand;
+  int n = sh.n_cand;
+  if (n > 2 * k + 64) {
+    // Ranking takes n steps a candidate: a bound among them first.
+#pragma unroll
+    for (int i = 0; i < kOwn; i++) {
+      const int c = int(threadIdx.x) + i * kScoreThreads;
+      own[i] = c < n ? sh.cand[c] : 0ull;
+    }
+    bound = key_bound(k, k + k / 2 + 16, 0ull, highest, [&](unsigned long long key) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; i++) c += own[i] >= key;
+      return cta_sum(c, turn, sh);
+    });
+    __syncthreads();  // every candidate is in registers
+    if (threadIdx.x == 0) sh.n_cand = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOwn; i++)
+      if (own[i] >= bound && own[i]) sh.cand[atomicAdd(&sh.n_cand, 1)] = own[i];
+    __syncthreads();
+    n = sh.n_cand;
+  }
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
     const unsigned long long mine = sh.cand[i];
     int rank = 0;
@@ -295,98 +396,96 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
   }
 }
 
-__global__ void __launch_bounds__(kScoreThreads) k_score(ScoreArgs a) {
+// The sets of `n` lanes joined, on every lane: lane pairs join the lower
+// lane's set first on both sides, so that all get the same bits.
+__device__ __forceinline__ Soft soft_lanes(Soft p, int n, int lane) {
+  for (int o = 1; o < n; o <<= 1) {
+    const Soft q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o),
+                 __shfl_xor_sync(0xffffffffu, p.t, o)};
+    p = (lane & o) ? soft_join(q, p) : soft_join(p, q);
+  }
+  return p;
+}
+// The sets of the CTA's warps (the same on each warp's lanes) joined, on every thread.
+__device__ __forceinline__ Soft soft_cta(const Soft& p, int warp, int lane, ScoreShared& sh) {
+  if (lane == 0) sh.soft[warp] = p;
+  __syncthreads();
+  return soft_lanes(sh.soft[lane % kScoreWarps], kScoreWarps, lane);
+}
+
+__global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
   __shared__ ScoreShared sh;
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t row = blockIdx.x / unsigned(a.chunks);
-  const int chunk = int(blockIdx.x % unsigned(a.chunks));
-  const Row r(a.logits, row, a.vocab);
-  int* block_max = a.top ? a.block_max + row * size_t(a.max_blocks) : nullptr;
-  const int b0 = chunk * a.chunk_blocks, b1 = min(r.blocks, b0 + a.chunk_blocks);
-  Soft s{-INFINITY, 0.f, 0.f};
-  for (int b = b0 + warp * kUnroll; b < b1; b += kScoreWarps * kUnroll) {
-    float4 v[kUnroll];
-    bool in[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      in[u] = b + u < b1 && r.inside(b + u);
-      if (in[u]) v[u] = r.load(b + u, lane);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      if (b + u >= b1) break;
-      int bm;
-      if (in[u]) {
-        bm = max4(v[u]);
-      } else {
-        v[u] = r.load_end(b + u, lane, __int_as_float(-1));  // the lowest in order
-        bm = max4(v[u]);
-        v[u] = r.load_end(b + u, lane, -INFINITY);
-      }
-      bm = __reduce_max_sync(0xffffffffu, bm);
-      if (block_max && lane == 0) block_max[b + u] = bm;
-      add_block(s, v[u], bm, lane);
-    }
-  }
-  s.s = warp_sum(s.s);
-  s.t = warp_sum(s.t);
-  if (lane == 0) sh.soft[warp] = s;
-  __syncthreads();
-  s = sh.soft[0];
-#pragma unroll
-  for (int w = 1; w < kScoreWarps; w++) s = soft_join(s, sh.soft[w]);
-  if (a.chunks > 1) {
-    if (threadIdx.x == 0) {
-      a.part[blockIdx.x] = make_float4(s.m, s.s, s.t, 0.f);
-      __threadfence();
-      sh.last = atomicAdd(a.ticket + row, 1u) == unsigned(a.chunks) - 1;
-      __threadfence();
-    }
-    __syncthreads();
-    if (!sh.last) return;
-    // The last CTA of the row: every chunk's sums, in an order that is the same each time.
-    Soft p{-INFINITY, 0.f, 0.f};
-    for (int c = threadIdx.x; c < a.chunks; c += kScoreThreads) {
-      const float4 q = __ldcg(a.part + row * a.chunks + c);
-      p = soft_join(p, Soft{q.x, q.y, q.z});
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Soft q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o),
-                   __shfl_xor_sync(0xffffffffu, p.t, o)};
-      // The lower lane's set first on both sides, so that both get the same bits.
-      p = (lane & o) ? soft_join(q, p) : soft_join(p, q);
-    }
-    if (lane == 0) sh.soft[warp] = p;
-    __syncthreads();
-    s = sh.soft[0];
-#pragma unroll
-    for (int w = 1; w < kScoreWarps; w++) s = soft_join(s, sh.soft[w]);
-    if (threadIdx.x == 0) a.ticket[row] = 0;
-  }
   const float nan = __int_as_float(0x7FC00000);
-  const bool bad = !(s.m < INFINITY) || s.m == -INFINITY || isnan(s.s);
-  const float logz = bad ? nan : log1pf(s.s);
-  if (threadIdx.x == 0) {
-    a.entropy[row] = logz + kLn2 * s.t / (1.0f + s.s);
-    const uint32_t tok = a.tokens[row];
-    a.logprob[row] = tok < uint32_t(a.vocab) ? (__ldg(r.base + r.shift + tok) - s.m) - logz : nan;
+  long long g = blockIdx.x * a.run;
+  const long long g1 = min(a.total, g + a.run);
+  while (g < g1) {
+    const size_t row = size_t(g / a.steps);
+    const int s0 = int(g - (long long)row * a.steps), s1 = int(min((long long)a.steps, s0 + (g1 - g)));
+    g += s1 - s0;
+    const Row r(a.logits, row, a.vocab);
+    int* block_max = a.top ? a.block_max + row * size_t(a.steps) * kStep : nullptr;
+    // The token's logit, for whoever finishes the row: on its way while the others are read.
+    float given = nan;
+    if (threadIdx.x == 0) {
+      const uint32_t tok = a.tokens[row];
+      if (tok < uint32_t(a.vocab)) given = __ldg(r.base + r.shift + tok);
+    }
+    Running run;
+    for (int st = s0 + warp; st < s1; st += kScoreWarps) {
+      const int b = st * kStep;
+      const bool whole = r.inside(b) && r.inside(b + kStep - 1);
+      float4 v[kStep];
+      int bm[kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; u++) v[u] = whole ? r.load(b + u, lane) : r.load_end(b + u, lane, -INFINITY);
+      add_step(run, v, bm, lane, whole, [&](int u, int j) {
+        const int at = r.element(b + u, lane, j);
+        return whole || (at >= 0 && at < a.vocab);
+      });
+      if (block_max && lane == 0) reinterpret_cast<int4*>(block_max)[st] = make_int4(bm[0], bm[1], bm[2], bm[3]);
+    }
+    Soft s = run.settled();
+    s.s = warp_sum(s.s);
+    s.t = warp_sum(s.t);
+    s = soft_cta(s, warp, lane, sh);
+    // Pieces of this row: those of the CTAs whose runs meet it.
+    const long long c0 = (long long)row * a.steps / a.run, c1 = ((long long)(row + 1) * a.steps - 1) / a.run;
+    if (c1 > c0) {
+      if (threadIdx.x == 0) {
+        a.part[row + blockIdx.x] = make_float4(s.m, s.s, s.t, 0.f);
+        unsigned before;  // releases this CTA's writes, acquires those of the CTAs before it
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.ticket + row) : "memory");
+        sh.last = before == unsigned(c1 - c0);
+      }
+      __syncthreads();
+      if (!sh.last) {
+        __syncthreads();  // sh.last is read before the next piece writes it
+        continue;
+      }
+      Soft p{-INFINITY, 0.f, 0.f};
+      for (long long c = c0 + threadIdx.x; c <= c1; c += kScoreThreads) {
+        const float4 q = __ldcg(a.part + row + c);
+        p = soft_join(p, Soft{q.x, q.y, q.z});
+      }
+      s = soft_cta(soft_lanes(p, 32, lane), warp, lane, sh);
+      if (threadIdx.x == 0) a.ticket[row] = 0;
+    }
+    const bool bad = !(s.m < INFINITY) || s.m == -INFINITY || isnan(s.s);
+    const float logz = bad ? nan : log1pf(s.s);
+    if (threadIdx.x == 0) {
+      a.entropy[row] = logz + kLn2 * s.t / (1.0f + s.s);
+      a.logprob[row] = (given - s.m) - logz;
+    }
+    if (a.top) alternatives(a, r, row, block_max, s.m, logz, sh);
+    __syncthreads();  // shared memory is free for the next piece
   }
-  if (a.top) alternatives(a, r, row, block_max, s.m, logz, sh);
 }
 
-// Blocks of a row, whatever its alignment.
-int score_blocks(size_t vocab) { return int((vocab + 3 + kBlock - 1) / kBlock); }
-// CTAs that a call of n rows aims for: eight resident ones on each SM.
-int score_target(const tb200_device* d) { return 8 * d->sms; }
-// Chunks per row: one when the rows alone fill the GPU; else enough to, each
-// of at least one block for every warp.
-int score_chunks(const tb200_device* d, size_t n, int blocks) {
-  const size_t want = (size_t(score_target(d)) + n - 1) / n;
-  return int(std::max<size_t>(1, std::min<size_t>(want, size_t(blocks + kScoreWarps - 1) / kScoreWarps)));
-}
+// Steps of a row, whatever its alignment.
+int score_steps(size_t vocab) { return int((vocab + 3 + kStep * kBlock - 1) / (kStep * kBlock)); }
 
 }  // namespace
 }  // namespace tb
@@ -404,14 +503,16 @@ int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, t
   s->rows = rows;
   s->vocab = vocab;
   s->top = int(top);
-  cudaError_t e = cudaMalloc(&s->logprob, rows * 4);
+  const size_t blocks = size_t(tb::score_steps(vocab)) * tb::kStep;
+  int per_sm = 0;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, tb::k_score, tb::kScoreThreads, 0);
+  s->ctas = std::max(1, per_sm) * dev->sms;
+  const size_t parts = rows + size_t(s->ctas);
+  if (e == cudaSuccess) e = cudaMalloc(&s->logprob, rows * 4);
   if (e == cudaSuccess) e = cudaMalloc(&s->entropy, rows * 4);
   if (e == cudaSuccess) e = cudaMalloc(&s->tokens, rows * 4);
   if (e == cudaSuccess && top) e = cudaMalloc(&s->top_ids, rows * top * 4);
   if (e == cudaSuccess && top) e = cudaMalloc(&s->top_logprobs, rows * top * 4);
-  const int blocks = tb::score_blocks(vocab);
-  // n rows in score_chunks(n) chunks: at most n + the CTAs aimed for, and no row has more than blocks.
-  const size_t parts = rows + size_t(tb::score_target(dev));
   if (e == cudaSuccess) e = cudaMalloc(&s->part, parts * sizeof(float4));
   if (e == cudaSuccess) e = cudaMalloc(&s->ticket, rows * 4);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->ticket, 0, rows * 4, dev->stream);
@@ -481,11 +582,11 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.ticket = s->ticket;
   a.vocab = int(s->vocab);
   a.top = s->top;
-  a.max_blocks = tb::score_blocks(s->vocab);
-  a.chunks = tb::score_chunks(s->dev, n, a.max_blocks);
-  a.chunk_blocks = (a.max_blocks + a.chunks - 1) / a.chunks;
-  a.chunks = (a.max_blocks + a.chunk_blocks - 1) / a.chunk_blocks;
-  tb::launch_pdl(tb::k_score, dim3(unsigned(n * a.chunks)), dim3(tb::kScoreThreads), 0, st, a);
+  a.steps = tb::score_steps(s->vocab);
+  a.total = (long long)n * a.steps;
+  // Equal runs for the CTAs that run at once.
+  a.run = (a.total + s->ctas - 1) / s->ctas;
+  tb::launch_pdl(tb::k_score, dim3(unsigned((a.total + a.run - 1) / a.run)), dim3(tb::kScoreThreads), 0, st, a);
   return rt::launched("score");
 }
 
