@@ -16,13 +16,19 @@
 // (whatever the number of rows, no SM waits for another's last row); a CTA's
 // part of a row is a piece. A warp takes a step at a time, as four blocks of
 // 128: their largest, a redux each, are both the running maximum that the sums
-// refer to, so that rescaling is a rare warp-uniform branch, and the blocks'
-// entries in a table of 1/128 of the logits' size. Per logit that leaves five
-// instructions for the sums and one for the maximum; at ten it was bound by
-// them (1111 x 151936: 142 us, against 105 us for the bytes). The CTA that finishes a row's last piece joins the pieces'
-// sums, in their order, and finds the alternatives: the k largest logits lie in
-// the k blocks with the largest maxima (each of those has an element at least as
-// large as any element of another block), so only those blocks are read again.
+// refer to and the blocks' entries in a table of 1/128 of the logits' size. The
+// warps of a CTA begin a piece with the largest of their first steps as common
+// maximum, so that few steps raise it: that takes a warp-uniform branch as
+// dear as the step itself. Per logit there are five instructions for the sums
+// and one for the maximum; at ten it was bound by them (1111 x 151936: 142 us,
+// against 105 us for the bytes). The CTA that finishes a row's last piece joins the pieces'
+// sums, in their order. The alternatives: the k largest logits lie in the k blocks
+// with the largest maxima (each of those has an element at least as large as any
+// element of another block), so only those are read again; the same goes for
+// the granules of four logits among them. That is a few microseconds a row of
+// waiting more than of work: with few rows the CTA that finishes a row does it,
+// with many it is a kernel of its own with a CTA for every row (1111 rows, one
+// alternative: 131 us in one kernel, of which 20 are theirs).
 #include <algorithm>
 #include <climits>
 #include <string>
@@ -38,6 +44,7 @@ struct tb200_scorer {
   uint32_t* tokens = nullptr;   // [rows] ids given in host memory
   float4* part = nullptr;       // sums of the pieces
   int* block_max = nullptr;     // [rows][a row's blocks], when there are alternatives
+  float2* peak = nullptr;       // [rows] maximum and log Z, when there are alternatives
   unsigned* ticket = nullptr;   // [rows], zero between launches
   int ctas = 0;                 // that the GPU runs at once
 };
@@ -50,9 +57,13 @@ constexpr int kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreMaxTop = 64;
 constexpr int kBlock = 128;        // logits per table entry
 constexpr int kStep = 4;           // blocks a warp takes at a time
-constexpr int kCand = 2048;        // candidates held in shared memory
-constexpr int kOwn = 8;            // table entries or candidates a thread keeps in registers
-static_assert(kCand == kOwn * kScoreThreads, "a thread's candidates fit its registers");
+// Alternatives: a search for the k largest may end with up to this many.
+__host__ __device__ constexpr int slack(int k) { return k + k / 2 + 4; }
+constexpr int kPicked = slack(kScoreMaxTop);  // blocks read again
+constexpr int kCand = 4 * kPicked;            // elements of as many granules
+constexpr int kOwn = 8;                       // table entries a thread keeps in registers
+constexpr int kGranules = 13;                 // granules of the picked blocks that it keeps
+static_assert(kPicked * 32 <= kGranules * kScoreThreads, "they fit");
 constexpr int kNegInf = int(0xFF800000u ^ 0x7FFFFFFFu);  // order(-inf)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -73,24 +84,24 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The softmax of a set of logits: its largest m, and the sums above over the
-// others; t in units of log 2. An empty set has m = -inf.
+// The softmax of a set of logits under a maximum m that none of them exceeds:
+// the sums above, t in units of log 2. own: 1 where m is one of the set's logits,
+// which then stands outside the sums, else 0. An empty set may have m = -inf.
 struct Soft {
-  float m, s, t;
+  float m, s, t, own;
 };
-// `a` seen from a larger maximum m: its own largest joins the others.
-__device__ __forceinline__ Soft soft_under(const Soft a, float m) {
-  const float d = (m - a.m) * kLog2e, e = ex2(-d);
-  if (e == 0.0f) return Soft{m, 0.0f, 0.0f};  // d may be infinite
-  const float s = fmaf(e, a.s, e);
-  return Soft{m, s, fmaf(e, a.t, d * s)};
-}
 __device__ __forceinline__ Soft soft_join(const Soft a, const Soft b) {
   const bool a_big = !(b.m > a.m);
   const Soft hi = a_big ? a : b, lo = a_big ? b : a;
-  if (lo.m == -INFINITY) return Soft{hi.m, hi.s + lo.s, hi.t};  // nothing, or the NaN that it met
-  const Soft u = soft_under(lo, hi.m);
-  return Soft{hi.m, hi.s + u.s, hi.t + u.t};
+  if (lo.m == -INFINITY) return Soft{hi.m, hi.s + lo.s, hi.t, hi.own};  // nothing, or the NaN that it met
+  const float d = (hi.m - lo.m) * kLog2e, e = ex2(-d);
+  if (d == 0.0f) {  // of two places of the maximum one stays outside
+    const float own = fmaxf(hi.own, lo.own);
+    return Soft{hi.m, hi.s + lo.s + (hi.own + lo.own - own), hi.t + lo.t, own};
+  }
+  if (e == 0.0f) return Soft{hi.m, hi.s + lo.s * 0.0f, hi.t, hi.own};  // d may be infinite; a NaN stays
+  const float s = e * (lo.s + lo.own);
+  return Soft{hi.m, hi.s + s, hi.t + fmaf(e, lo.t, d * s), hi.own};
 }
 
 // The row as blocks of 128 logits that start on 16-byte boundaries: element
@@ -123,38 +134,40 @@ struct Row {
   }
 };
 
-// A warp's set while it grows: m is the warp's, s and t each lane's shares of
-// the sums, taken at c = f32(m log2 e) in the place of m log2 e, which saves an
-// instruction a logit: what that leaves out (lo) is put right in settled().
+// A warp's set while it grows: m and own are the warp's, s and t each lane's
+// shares of the sums, taken at c = f32(m log2 e) in the place of m log2 e, which
+// saves an instruction a logit: what that leaves out (lo) is put right in settled().
 struct Running {
   float m, c, lo, s, t;
   int order;  // of m
-  __device__ __forceinline__ Running() : m(-INFINITY), c(0.f), lo(0.f), s(0.f), t(0.f), order(kNegInf) {}
-  __device__ __forceinline__ Soft settled() const {
-    const float f = ex2(-lo);
-    return Soft{m, s * f, fmaf(lo, s, t) * f};
-  }
-  // Refers the sums to a larger maximum; lane 0 takes the old one's own term.
-  __device__ __forceinline__ void raise(int bm, int lane) {
-    const Soft old = settled();
-    const float nm = unorder(bm);
-    if (order > kNegInf) {
-      const float d = (nm - old.m) * kLog2e, e = ex2(-d);
-      if (e == 0.0f) {
-        s = old.s * 0.0f;  // a NaN stays
-        t = 0.0f;
-      } else {
-        s = lane == 0 ? fmaf(e, old.s, e) : e * old.s;
-        t = fmaf(e, old.t, d * s);
-      }
-    }
-    m = nm;
-    order = bm;
+  bool own;
+  __device__ __forceinline__ explicit Running(int o) : s(0.f), t(0.f), own(false) { refer(o); }
+  __device__ __forceinline__ void refer(int o) {
+    order = o;
+    m = unorder(o);
     c = m * kLog2e;
-    lo = huge() ? 0.f : fmaf(m, kLog2e, -c);
+    lo = m > -INFINITY && !huge() ? fmaf(m, kLog2e, -c) : 0.f;
   }
   // Whether m log2 e may be past f32's range.
   __device__ __forceinline__ bool huge() const { return fabsf(m) > 1e38f; }
+  __device__ __forceinline__ Soft settled() const {
+    const float f = ex2(-lo);
+    return Soft{m, s * f, fmaf(lo, s, t) * f, own ? 1.f : 0.f};
+  }
+  // Refers the sums to a larger maximum; lane 0 takes the old one's own term.
+  __device__ __forceinline__ void raise(int o, int lane) {
+    const Soft old = settled();
+    const int before = order;
+    refer(o);
+    const float d = (m - old.m) * kLog2e, e = ex2(-d);
+    if (before <= kNegInf || e == 0.0f) {
+      s = old.s * 0.0f;  // a NaN stays
+      t = 0.0f;
+    } else {
+      s = e * (own && lane == 0 ? old.s + 1.0f : old.s);
+      t = fmaf(e, old.t, d * s);
+    }
+  }
   // A logit's share of the sums. Far below the maximum (or excluded) it adds 0, not 0 * -inf.
   template <bool HUGE>
   __device__ __forceinline__ void add(float x) {
@@ -165,16 +178,15 @@ struct Running {
   }
 };
 
-// Four blocks: their largest in order go to bm, their sums to a. `real(u, j)`
-// is whether value j of block u is the row's (`whole`: all are).
+// The largest in order of each of four blocks, for the warp; the largest of
+// them. `real(u, j)`: value j of block u is the row's (`whole`: all are). nan:
+// set to a NaN that a lane meets.
 template <class Real>
-__device__ __forceinline__ void add_step(Running& a, float4 (&v)[kStep], int (&bm)[kStep], int lane, bool whole,
-                                         Real real) {
-  float x[kStep][4];
+__device__ __forceinline__ int step_max(const float (&x)[kStep][4], int (&bm)[kStep], float& nan, bool whole,
+                                        Real real) {
   float m[kStep], least = INFINITY;
 #pragma unroll
   for (int u = 0; u < kStep; u++) {
-    x[u][0] = v[u].x, x[u][1] = v[u].y, x[u][2] = v[u].z, x[u][3] = v[u].w;
     m[u] = x[u][0];
 #pragma unroll
     for (int j = 1; j < 4; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[u]) : "f"(x[u][j]));
@@ -191,21 +203,26 @@ __device__ __forceinline__ void add_step(Running& a, float4 (&v)[kStep], int (&b
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         if (real(u, j)) bm[u] = max(bm[u], order(x[u][j]));
-        if (isnan(x[u][j])) a.s = x[u][j];
+        if (isnan(x[u][j])) nan = x[u][j];
       }
     }
   }
   __syncwarp();
 #pragma unroll
   for (int u = 0; u < kStep; u++) bm[u] = __reduce_max_sync(0xffffffffu, bm[u]);
-  const int top = max(max(bm[0], bm[1]), max(bm[2], bm[3]));
-  if (top > a.order) {  // a new maximum, the same for the warp
-    a.raise(top, lane);
-    // It stays out of the sums itself: its first place in the step.
+  return max(max(bm[0], bm[1]), max(bm[2], bm[3]));
+}
+
+// Adds a step's logits, none above a.m, to the sums. With `leave`, the first
+// place of a.m in the step stays outside them.
+__device__ __forceinline__ void step_add(Running& a, float (&x)[kStep][4], int lane, bool leave) {
+  if (a.order <= kNegInf) return;  // nothing but excluded tokens so far
+  if (leave) {
+    a.own = true;
     int mine = kStep * 4;
 #pragma unroll
     for (int i = kStep * 4 - 1; i >= 0; i--)
-      if (order(x[i / 4][i % 4]) == top && real(i / 4, i % 4)) mine = i;
+      if (x[i / 4][i % 4] == a.m) mine = i;
     const unsigned who = __ballot_sync(0xffffffffu, mine < kStep * 4);
     if (lane == __ffs(who) - 1) {
 #pragma unroll
@@ -213,7 +230,6 @@ __device__ __forceinline__ void add_step(Running& a, float4 (&v)[kStep], int (&b
         if (i == mine) x[i / 4][i % 4] = -INFINITY;
     }
   }
-  if (a.order <= kNegInf) return;  // nothing but excluded tokens so far
   if (a.huge()) {
     for (int i = 0; i < kStep * 4; i++) a.add<true>(x[i / 4][i % 4]);
     return;
@@ -249,6 +265,7 @@ struct ScoreArgs {
   float4* part;     // piece of row r by CTA c: [r + c]
   int* block_max;   // [rows][steps * kStep]
   unsigned* ticket;
+  float2* peak;     // [rows] maximum and log Z for k_alternatives, or null
   int vocab, top;
   int steps;        // of a row, whatever its alignment
   long long total;  // steps of all rows
@@ -258,9 +275,11 @@ struct ScoreArgs {
 struct ScoreShared {
   Soft soft[kScoreWarps];
   int last, n_blocks, n_cand;
+  int first[kScoreWarps];
   int counts[2][kScoreWarps];
+  uint2 range[kScoreWarps];
   unsigned long long cand[kCand];
-  int blocks[kScoreMaxTop + kScoreMaxTop / 2 + 16];
+  int blocks[kPicked];
 };
 
 // The sum of c over the CTA, on every thread. Calls take `turn` 0, 1, 0, ... in
@@ -277,114 +296,149 @@ __device__ __forceinline__ int cta_sum(int c, int& turn, ScoreShared& sh) {
   return total;
 }
 
-// The `top` largest of the row, ranked: by the whole CTA.
-__device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const int* block_max, float m, float logz,
-                             ScoreShared& sh) {
+// A bound for the keys that the CTA's threads hold (N each, 0 for none; `held`,
+// at least k, in all): between k and slack(k) keys are at or above it.
+template <int N>
+__device__ __forceinline__ unsigned long long own_bound(int k, const unsigned long long (&own)[N], int held, int& turn,
+                                                        ScoreShared& sh) {
+  if (held <= slack(k)) return 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int k = a.top;
-  // No key is above this one. (m's sign is not relied on where it is zero.)
-  const unsigned long long highest = m > 0.0f && !isnan(logz) ? order_key(order(m), 0) : ~0ull;
-  int turn = 0;
-  if (threadIdx.x == 0) sh.n_blocks = sh.n_cand = 0;
-  unsigned long long own[kOwn];
-  // The blocks with the largest maxima: k of them, or more where that ends the search sooner.
+  // None is above the largest; where every thread has one, the least of the
+  // threads' largest has 256 >= k at or above it.
+  unsigned high = 0;
 #pragma unroll
-  for (int i = 0; i < kOwn; i++) {
-    const int b = int(threadIdx.x) + i * kScoreThreads;
-    own[i] = b < r.blocks ? order_key(__ldcg(block_max + b), uint32_t(b)) : 0ull;
-  }
-  const int kb = min(k, r.blocks);
-  // Where every thread has a block, the least of their largest has 256 >= k keys at or above it.
-  unsigned long long lo = 0;
-  if (r.blocks >= kScoreThreads) {
-    unsigned mine = 0;
-#pragma unroll
-    for (int i = 0; i < kOwn; i++) mine = max(mine, unsigned(own[i] >> 32));
-    mine = __reduce_min_sync(0xffffffffu, mine);
-    if (lane == 0) sh.counts[1][warp] = int(mine);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kScoreWarps; w++) mine = min(mine, unsigned(sh.counts[1][w]));
-    lo = static_cast<unsigned long long>(mine) << 32;
-  }
-  unsigned long long bound = key_bound(kb, kb + kb / 2 + 16, lo, highest, [&](unsigned long long key) {
+  for (int i = 0; i < N; i++) high = max(high, unsigned(own[i] >> 32));
+  const unsigned low = __reduce_min_sync(0xffffffffu, high);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) sh.range[warp] = make_uint2(low, high);
+  __syncthreads();
+  const uint2 w = sh.range[lane % kScoreWarps];
+  const unsigned long long lo = static_cast<unsigned long long>(__reduce_min_sync(0xffffffffu, w.x)) << 32;
+  const unsigned long long hi =
+      (static_cast<unsigned long long>(__reduce_max_sync(0xffffffffu, w.y)) << 32) | 0xFFFFFFFFull;
+  return max(1ull, key_bound(k, slack(k), lo, hi, [&](unsigned long long key) {
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kOwn; i++) c += own[i] >= key;
-    for (int b = int(threadIdx.x) + kOwn * kScoreThreads; b < r.blocks; b += kScoreThreads)
-      c += order_key(__ldcg(block_max + b), uint32_t(b)) >= key;
+    for (int i = 0; i < N; i++) c += own[i] >= key;
     return cta_sum(c, turn, sh);
-  });
-  __syncthreads();
-  auto pick = [&](unsigned long long key, int b) {
-    if (key >= bound && key) sh.blocks[atomicAdd(&sh.n_blocks, 1)] = b;
-  };
+  }));
+}
+
+// The keys of a lane's granule of block b (0 where it is not the row's).
+__device__ __forceinline__ void granule_keys(const Row& r, int b, int lane, float4 v, unsigned long long (&key)[4]) {
+  const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < kOwn; i++) pick(own[i], int(threadIdx.x) + i * kScoreThreads);
-  for (int b = int(threadIdx.x) + kOwn * kScoreThreads; b < r.blocks; b += kScoreThreads)
-    pick(order_key(__ldcg(block_max + b), uint32_t(b)), b);
-  __syncthreads();
-  const int nb = sh.n_blocks;
-  // f(key) of every element of those blocks.
-  auto each = [&](auto f) {
-    for (int i = warp; i < nb; i += kScoreWarps) {
-      const int b = sh.blocks[i];
-      const float4 v = r.inside(b) ? r.load(b, lane) : r.load_end(b, lane, 0.f);
-      const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int at = r.element(b, lane, j);
-        f(at >= 0 && at < a.vocab ? order_key(order(x[j]), uint32_t(at)) : 0ull);
-      }
-    }
-  };
-  auto collect = [&](unsigned long long least) {
-    each([&](unsigned long long key) {
-      if (key >= least && key) {
-        const int at = atomicAdd(&sh.n_cand, 1);
-        if (at < kCand) sh.cand[at] = key;
-      }
-    });
-    __syncthreads();
-  };
-  // Candidates: the elements at least as large as the smallest of the picked
-  // maxima (k of these exist), or all elements where there are fewer blocks than k.
-  collect(r.blocks < k ? 0ull : bound & 0xFFFFFFFF00000000ull);
-  if (sh.n_cand > kCand) {
-    // More than there is room for (neighbours that are all large): a bound that leaves fewer.
-    bound = key_bound(k, kCand, 0ull, highest, [&](unsigned long long key) {
-      int c = 0;
-      each([&](unsigned long long x) { c += x >= key; });
-      return cta_sum(c, turn, sh);
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n_cand = 0;
-    __syncthreads();
-    collect(bound);
+  for (int j = 0; j < 4; j++) {
+    const int at = r.element(b, lane, j);
+    key[j] = at >= 0 && at < r.vocab ? order_key(order(x[j]), uint32_t(at)) : 0ull;
   }
-  int n = sh.n_cand;
-  if (n > 2 * k + 64) {
-    // Ranking takes n steps a candidate: a bound among them first.
+}
+
+// Candidates among the listed blocks where too many elements pass the blocks'
+// bound (neighbours that are all large, or fewer blocks than k): the same search
+// among the blocks' granules, each the largest of four, leaves at most 4 slack(k).
+__device__ __noinline__ void granule_candidates(const Row& r, int k, int& turn, ScoreShared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nb = sh.n_blocks;
+  auto load = [&](int i, unsigned long long (&key)[4]) {
+    const int b = sh.blocks[i * kScoreWarps + warp];
+    granule_keys(r, b, lane, r.inside(b) ? r.load(b, lane) : r.load_end(b, lane, 0.f), key);
+  };
+  unsigned long long own[kGranules];
+  int held = 0;
+#pragma unroll
+  for (int i = 0; i < kGranules; i++) {
+    own[i] = 0;
+    if (i * kScoreWarps + warp < nb) {
+      unsigned long long key[4];
+      load(i, key);
+      own[i] = max(max(key[0], key[1]), max(key[2], key[3]));
+      held += own[i] != 0;
+    }
+  }
+  held = cta_sum(held, turn, sh);
+  const unsigned long long bound = own_bound(min(k, held), own, held, turn, sh);
+  const unsigned long long least = held < k ? 1ull : bound;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n_cand = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kGranules; i++) {
+    if (own[i] < bound) continue;
+    unsigned long long key[4];
+    load(i, key);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (key[j] >= least) sh.cand[atomicAdd(&sh.n_cand, 1)] = key[j];
+  }
+  __syncthreads();
+}
+
+// The `top` largest of a row with maximum m, ranked: by the whole CTA.
+__device__ __forceinline__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, float m, float logz,
+                                             ScoreShared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k = a.top;
+  const int* block_max = a.block_max + row * size_t(a.steps) * kStep;
+  int turn = 0;
+  if (threadIdx.x == 0) sh.n_blocks = sh.n_cand = 0;
+  // The blocks with the largest maxima: k of them, or more where that ends the search sooner.
+  auto block_key = [&](int b) { return order_key(__ldcg(block_max + b), uint32_t(b)); };
+  const int kb = min(k, r.blocks);
+  unsigned long long bound;
+  if (r.blocks <= kOwn * kScoreThreads) {
+    unsigned long long own[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; i++) {
-      const int c = int(threadIdx.x) + i * kScoreThreads;
-      own[i] = c < n ? sh.cand[c] : 0ull;
+      const int b = int(threadIdx.x) + i * kScoreThreads;
+      own[i] = b < r.blocks ? block_key(b) : 0ull;
     }
-    bound = key_bound(k, k + k / 2 + 16, 0ull, highest, [&](unsigned long long key) {
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < kOwn; i++) c += own[i] >= key;
-      return cta_sum(c, turn, sh);
-    });
-    __syncthreads();  // every candidate is in registers
-    if (threadIdx.x == 0) sh.n_cand = 0;
+    bound = own_bound(kb, own, r.blocks, turn, sh);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; i++)
-      if (own[i] >= bound && own[i]) sh.cand[atomicAdd(&sh.n_cand, 1)] = own[i];
+      if (own[i] >= bound) sh.blocks[atomicAdd(&sh.n_blocks, 1)] = int(threadIdx.x) + i * kScoreThreads;
+  } else {
+    bound = key_bound(k, slack(k), 0ull, ~0ull, [&](unsigned long long key) {
+      int c = 0;
+      for (int b = threadIdx.x; b < r.blocks; b += kScoreThreads) c += block_key(b) >= key;
+      return cta_sum(c, turn, sh);
+    });
     __syncthreads();
-    n = sh.n_cand;
+    for (int b = threadIdx.x; b < r.blocks; b += kScoreThreads)
+      if (block_key(b) >= bound) sh.blocks[atomicAdd(&sh.n_blocks, 1)] = b;
   }
+  __syncthreads();
+  const int nb = sh.n_blocks;
+  // Candidates: the elements at least as large as the smallest of the picked maxima (k of these exist).
+  const bool all = r.blocks <= slack(kb);  // no bound was needed
+  if (!all) {
+    const unsigned long long least = bound & 0xFFFFFFFF00000000ull;
+    constexpr int kBatch = 4;
+    for (int i0 = warp; i0 < nb; i0 += kBatch * kScoreWarps) {
+      float4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (i0 + i * kScoreWarps < nb) {
+          const int b = sh.blocks[i0 + i * kScoreWarps];
+          v[i] = r.inside(b) ? r.load(b, lane) : r.load_end(b, lane, 0.f);
+        }
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (i0 + i * kScoreWarps < nb) {
+          unsigned long long key[4];
+          granule_keys(r, sh.blocks[i0 + i * kScoreWarps], lane, v[i], key);
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (key[j] >= least && key[j]) {
+              const int at = atomicAdd(&sh.n_cand, 1);
+              if (at < kCand) sh.cand[at] = key[j];
+            }
+        }
+    }
+    __syncthreads();
+  }
+  if (all || sh.n_cand > kCand) granule_candidates(r, k, turn, sh);
+  const int n = sh.n_cand;
   for (int i = threadIdx.x; i < n; i += kScoreThreads) {
     const unsigned long long mine = sh.cand[i];
     int rank = 0;
@@ -401,7 +455,7 @@ __device__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, const
 __device__ __forceinline__ Soft soft_lanes(Soft p, int n, int lane) {
   for (int o = 1; o < n; o <<= 1) {
     const Soft q{__shfl_xor_sync(0xffffffffu, p.m, o), __shfl_xor_sync(0xffffffffu, p.s, o),
-                 __shfl_xor_sync(0xffffffffu, p.t, o)};
+                 __shfl_xor_sync(0xffffffffu, p.t, o), __shfl_xor_sync(0xffffffffu, p.own, o)};
     p = (lane & o) ? soft_join(q, p) : soft_join(p, q);
   }
   return p;
@@ -413,7 +467,7 @@ __device__ __forceinline__ Soft soft_cta(const Soft& p, int warp, int lane, Scor
   return soft_lanes(sh.soft[lane % kScoreWarps], kScoreWarps, lane);
 }
 
-__global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
+__global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
   __shared__ ScoreShared sh;
   pdl_launch_dependents();
   pdl_wait();
@@ -433,20 +487,41 @@ __global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
       const uint32_t tok = a.tokens[row];
       if (tok < uint32_t(a.vocab)) given = __ldg(r.base + r.shift + tok);
     }
-    Running run;
-    for (int st = s0 + warp; st < s1; st += kScoreWarps) {
+    int st = s0 + warp;
+    bool whole = false;
+    float x[kStep][4], met = 0.f;
+    int bm[kStep], top = INT_MIN;
+    auto load = [&] {
       const int b = st * kStep;
-      const bool whole = r.inside(b) && r.inside(b + kStep - 1);
-      float4 v[kStep];
-      int bm[kStep];
+      whole = r.inside(b) && r.inside(b + kStep - 1);
 #pragma unroll
-      for (int u = 0; u < kStep; u++) v[u] = whole ? r.load(b + u, lane) : r.load_end(b + u, lane, -INFINITY);
-      add_step(run, v, bm, lane, whole, [&](int u, int j) {
+      for (int u = 0; u < kStep; u++) {
+        const float4 v = whole ? r.load(b + u, lane) : r.load_end(b + u, lane, -INFINITY);
+        x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+      }
+      top = step_max(x, bm, met, whole, [&](int u, int j) {
         const int at = r.element(b + u, lane, j);
         return whole || (at >= 0 && at < a.vocab);
       });
       if (block_max && lane == 0) reinterpret_cast<int4*>(block_max)[st] = make_int4(bm[0], bm[1], bm[2], bm[3]);
+    };
+    if (st < s1) load();
+    if (lane == 0) sh.first[warp] = top;
+    __syncthreads();
+    int common = sh.first[lane % kScoreWarps];
+    const unsigned holders = __ballot_sync(0xffffffffu, common == __reduce_max_sync(0xffffffffu, common));
+    common = __shfl_sync(0xffffffffu, common, __ffs(holders) - 1);
+    Running run(max(common, kNegInf));
+    if (st < s1) {
+      step_add(run, x, lane, warp == __ffs(holders) - 1);
+      for (st += kScoreWarps; st < s1; st += kScoreWarps) {
+        load();
+        const bool higher = top > run.order;
+        if (higher) run.raise(top, lane);
+        step_add(run, x, lane, higher);
+      }
     }
+    run.s += met * 0.0f;  // a NaN stays
     Soft s = run.settled();
     s.s = warp_sum(s.s);
     s.t = warp_sum(s.t);
@@ -455,7 +530,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
     const long long c0 = (long long)row * a.steps / a.run, c1 = ((long long)(row + 1) * a.steps - 1) / a.run;
     if (c1 > c0) {
       if (threadIdx.x == 0) {
-        a.part[row + blockIdx.x] = make_float4(s.m, s.s, s.t, 0.f);
+        a.part[row + blockIdx.x] = make_float4(s.m, s.s, s.t, s.own);
         unsigned before;  // releases this CTA's writes, acquires those of the CTAs before it
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.ticket + row) : "memory");
         sh.last = before == unsigned(c1 - c0);
@@ -465,10 +540,10 @@ __global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
         __syncthreads();  // sh.last is read before the next piece writes it
         continue;
       }
-      Soft p{-INFINITY, 0.f, 0.f};
+      Soft p{-INFINITY, 0.f, 0.f, 0.f};
       for (long long c = c0 + threadIdx.x; c <= c1; c += kScoreThreads) {
         const float4 q = __ldcg(a.part + row + c);
-        p = soft_join(p, Soft{q.x, q.y, q.z});
+        p = soft_join(p, Soft{q.x, q.y, q.z, q.w});
       }
       s = soft_cta(soft_lanes(p, 32, lane), warp, lane, sh);
       if (threadIdx.x == 0) a.ticket[row] = 0;
@@ -479,9 +554,23 @@ __global__ void __launch_bounds__(kScoreThreads, 5) k_score(ScoreArgs a) {
       a.entropy[row] = logz + kLn2 * s.t / (1.0f + s.s);
       a.logprob[row] = (given - s.m) - logz;
     }
-    if (a.top) alternatives(a, r, row, block_max, s.m, logz, sh);
+    if (a.peak) {
+      if (threadIdx.x == 0) a.peak[row] = make_float2(s.m, logz);
+    } else if (a.top) {
+      alternatives(a, r, row, s.m, logz, sh);
+    }
     __syncthreads();  // shared memory is free for the next piece
   }
+}
+
+// The alternatives of row blockIdx.x.
+__global__ void __launch_bounds__(kScoreThreads, 4) k_alternatives(ScoreArgs a) {
+  __shared__ ScoreShared sh;
+  pdl_launch_dependents();
+  pdl_wait();
+  const size_t row = blockIdx.x;
+  const float2 p = a.peak[row];
+  alternatives(a, Row(a.logits, row, a.vocab), row, p.x, p.y, sh);
 }
 
 // Steps of a row, whatever its alignment.
@@ -517,6 +606,7 @@ int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, t
   if (e == cudaSuccess) e = cudaMalloc(&s->ticket, rows * 4);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->ticket, 0, rows * 4, dev->stream);
   if (e == cudaSuccess && top) e = cudaMalloc(&s->block_max, rows * blocks * 4);
+  if (e == cudaSuccess && top) e = cudaMalloc(&s->peak, rows * sizeof(float2));
   if (e == cudaSuccess) e = cudaMemsetAsync(s->logprob, 0, rows * 4, dev->stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->entropy, 0, rows * 4, dev->stream);
   if (e == cudaSuccess && top) e = cudaMemsetAsync(s->top_ids, 0, rows * top * 4, dev->stream);
@@ -541,6 +631,7 @@ int tb200_scorer_free(tb200_scorer* s) {
   cudaFree(s->top_logprobs);
   cudaFree(s->part);
   cudaFree(s->block_max);
+  cudaFree(s->peak);
   cudaFree(s->ticket);
   delete s;
   return TB200_OK;
@@ -584,9 +675,12 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.top = s->top;
   a.steps = tb::score_steps(s->vocab);
   a.total = (long long)n * a.steps;
-  // Equal runs for the CTAs that run at once.
-  a.run = (a.total + s->ctas - 1) / s->ctas;
+  // Equal runs for the CTAs that run at once, of a step for every warp at least where rows are that long.
+  a.run = std::max<long long>((a.total + s->ctas - 1) / s->ctas, std::min(a.steps, tb::kScoreWarps));
+  // More rows than half the CTAs: some would find alternatives while others wait for the rest of their run.
+  a.peak = 2 * n > size_t(s->ctas) ? s->peak : nullptr;
   tb::launch_pdl(tb::k_score, dim3(unsigned((a.total + a.run - 1) / a.run)), dim3(tb::kScoreThreads), 0, st, a);
+  if (a.peak) tb::launch_pdl(tb::k_alternatives, dim3(unsigned(n)), dim3(tb::kScoreThreads), 0, st, a);
   return rt::launched("score");
 }
 
