@@ -26,7 +26,7 @@ struct RowArgs {
   const void* x;      // [rows][cols] f32 (bf16: kRowBf16); kRowAddNorm: also written
   const float* y;     // kRowAddNorm: [rows][cols]
   const uint16_t* w;  // norm weight [cols]
-  double eps;
+  double eps, inv_cols;
   int8_t* q;          // [rows][ld]
   float* scale;       // [rows]
   int cols, ld;
@@ -37,37 +37,37 @@ __device__ __forceinline__ unsigned long long abs_bits(double v) {
   return static_cast<unsigned long long>(__double_as_longlong(v)) & 0x7FFFFFFFFFFFFFFFull;
 }
 
-// What a row's values have in common: the factor r that each is multiplied
-// by, the scale, and r / scale.
+// What a row's values have in common: the factor r that each is multiplied by
+// and the scale.
 struct RowScale {
-  double r, step, c;
-  float c32;
-  bool zero;  // every integer is 0 (a zero or non-finite row)
-  bool fast;  // c32 can be used: nothing near f32's limits
+  double r, c;      // c: r / s to a few units of 2^-48
+  float s;
+  float c32, sure;  // f32 products with c32 this near to an integer round as they have to
 };
-__device__ __forceinline__ RowScale row_scale(unsigned long long amax_bits, double r, float* scale_out) {
+__device__ __forceinline__ RowScale row_scale(double amax, double r) {
   RowScale k;
-  const double amax = __longlong_as_double(static_cast<long long>(amax_bits));
-  float s = float(amax * r / 127.0);
-  if (!(s <= 3.402823466e38f)) s = __int_as_float(0x7FC00000);  // NaN for NaN and infinity
-  *scale_out = s;
   k.r = r;
-  k.zero = !(s > 0.0f);
-  k.step = double(s);
-  k.c = k.zero ? 0.0 : r / k.step;
+  // The product with 1 / 127 is within 2^-52 of the quotient. Of an f32 amax (r = 1) the quotient
+  // is never that near to the middle of two f32 values, so its rounding is the quotient's.
+  k.s = float(amax * r * (1.0 / 127.0));
+  if (!(k.s <= 3.402823466e38f)) k.s = __int_as_float(0x7FC00000);  // NaN for NaN and infinity
+  const bool plain = amax > 0x1p-100 && amax < 0x1p100 && k.s > 0x1p-100f && k.s < 0x1p100f;
+  // One Newton step from the f32 reciprocal, which a division in 64 bits would take three of.
+  const double s = plain ? double(k.s) : 1.0, i = double(__frcp_rn(float(s)));
+  k.c = r * fma(i, fma(-s, i, 1.0), i);
   k.c32 = float(k.c);
-  k.fast = k.zero || (amax > 0x1p-100 && amax < 0x1p100 && s > 0x1p-100f);
+  k.sure = plain ? 0.49995f : -1.0f;  // near f32's limits every integer is computed by a quotient
   return k;
 }
-// The integer of a value v (before the factor r): rint(v r / step), by a product
-// with r / step except next to the middle of two integers, where the
-// product's last bits would decide.
+// rint(v r / s), the integer of a value v (before the factor r), in 64 bits.
+__device__ __noinline__ int row_int(double v, double r, float s) {
+  if (!(s > 0.0f)) return 0;  // zeros, or no numbers
+  return int(fmin(fmax(rint(v * r / double(s)), -127.0), 127.0));
+}
+// The same by a product, except next to the middle of two integers.
 __device__ __forceinline__ int row_int(double v, const RowScale& k) {
-  const double d = v * k.c;
-  double q = rint(d);
-  if (fabs(fabs(d - q) - 0.5) < 1e-9) q = rint(v * k.r / k.step);
-  q = fmin(fmax(q, -127.0), 127.0);
-  return k.zero ? 0 : int(q);
+  const double d = v * k.c, q = rint(d);
+  return k.sure > 0.f && fabs(fabs(d - q) - 0.5) > 1e-9 ? int(q) : row_int(v, k.r, k.s);
 }
 
 // Four consecutive values of a row of f32 or bf16, zeros past its end. With
@@ -99,129 +99,165 @@ __device__ __forceinline__ void store4(float* p, int left, float4 v) {
   }
 }
 
-// A row per `warps` warps (blockDim.x = 32 warps, blockDim.y rows a block),
-// E groups of four values a thread, held in registers between the pass that
-// finds the scale and the one that rounds.
+// The largest of |a| and b, a NaN if there is one.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(b));
+  return r;
+}
+// The largest of the lanes' bit patterns (f32 >= 0, or their halves) and of 64-bit ones.
+__device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
+  const unsigned hi = __reduce_max_sync(0xffffffffu, unsigned(v >> 32));
+  const unsigned lo = __reduce_max_sync(0xffffffffu, unsigned(v >> 32) == hi ? unsigned(v) : 0u);
+  return (static_cast<unsigned long long>(hi) << 32) | lo;
+}
+
+// The most threads of a block, by its threads' groups: what leaves them the registers.
+__host__ __device__ constexpr int row_threads(int e) { return e == 8 ? 512 : e == 4 ? 640 : 1024; }
+
+// A row per blockDim.x / 32 warps (blockDim.y rows a block), E groups of four
+// values a thread, held in registers between the pass that finds the scale and
+// the one that rounds.
 //
-// What bounds it is memory, so the 64-bit work is kept small: only the sum of
+// Every warp of a row repeats what a row costs beside its values (the two
+// reductions, the constants): 5003 x 2560 with the residual takes 46, 33 and
+// 30 us with one, two and four groups a thread.
+//
+// What should bound it is memory, so the 64-bit work is kept small (with all of
+// it in 64 bits the kernel took 51 instructions a value): only the sum of
 // squares takes a conversion per value. The largest |h w| is found among the
-// f32 products first (rounding keeps order), then exactly among the few that
-// round to it. The integers come from f32 products, whose error is below
-// 127 * 2^-22 = 3.1e-5 of a step (three roundings and c32's); only a value
+// f32 products first (rounding keeps order), then exactly by the threads that
+// hold it. The integers come from f32 products, whose error is below 127 * 2^-22
+// = 3.1e-5 of a step (h w, the product and c32 round once each); only a value
 // that near to the middle of two integers is computed again in 64 bits.
 template <int SRC, int E, bool VEC>
-__global__ void __launch_bounds__(1024) k_rows_q8(RowArgs a, long long rows) {
+__global__ void __launch_bounds__(row_threads(E)) k_rows_q8(RowArgs a, long long rows) {
   constexpr bool kNorm = SRC == kRowNorm || SRC == kRowAddNorm;
   __shared__ double red_s[32];
-  __shared__ unsigned long long red_m[32];
+  __shared__ unsigned red_m[32];
+  __shared__ unsigned long long exact;
   pdl_launch_dependents();
-  pdl_wait();
-  const int tid = threadIdx.x, warps = blockDim.x >> 5;
+  const int tid = threadIdx.x, warps = blockDim.x >> 5, lane = tid & 31;
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (tid == 0 && warps > 1) exact = 0;
+  pdl_wait();
   if (row >= rows) return;  // only where a row is one warp: no barrier below
   const float* xf = static_cast<const float*>(a.x) + row * a.cols;
   const uint16_t* xh = static_cast<const uint16_t*>(a.x) + row * a.cols;
 
-  float4 h[E];
+  float4 h[E], y[E];
   uint2 w[E];  // bf16
 #pragma unroll
   for (int i = 0; i < E; i++) {
     const int at = 4 * (tid + i * blockDim.x), left = a.cols - at;
-    h[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    h[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     w[i] = make_uint2(0, 0);
     if (left <= 0) continue;
     if constexpr (SRC == kRowBf16)
       h[i] = widen(load4<VEC>(xh + at, left));
     else
       h[i] = load4<VEC>(xf + at, left);
+    if constexpr (SRC == kRowAddNorm) y[i] = load4<VEC>(a.y + row * a.cols + at, left);
     if constexpr (kNorm) w[i] = load4<VEC>(a.w + at, left);
   }
-  if constexpr (SRC == kRowAddNorm) {
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-      const int at = 4 * (tid + i * blockDim.x), left = a.cols - at;
-      if (left <= 0) continue;
-      const float4 y = load4<VEC>(a.y + row * a.cols + at, left);
-      h[i] = make_float4(__fadd_rn(h[i].x, y.x), __fadd_rn(h[i].y, y.y), __fadd_rn(h[i].z, y.z),
-                         __fadd_rn(h[i].w, y.w));
-      store4<VEC>(const_cast<float*>(xf) + at, left, h[i]);
-    }
-  }
-
+  // What is rounded, before the row's factor: h w in f32, or the value itself.
+  auto products = [&](int i, float (&p)[4]) {
+    const float4 u = kNorm ? widen(w[i]) : make_float4(1.f, 1.f, 1.f, 1.f);
+    p[0] = kNorm ? __fmul_rn(h[i].x, u.x) : h[i].x;
+    p[1] = kNorm ? __fmul_rn(h[i].y, u.y) : h[i].y;
+    p[2] = kNorm ? __fmul_rn(h[i].z, u.z) : h[i].z;
+    p[3] = kNorm ? __fmul_rn(h[i].w, u.w) : h[i].w;
+  };
+  // The same exactly.
+  auto value = [&](int i, int j) {
+    const float4 u = kNorm ? widen(w[i]) : make_float4(1.f, 1.f, 1.f, 1.f);
+    const float v[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, f[4] = {u.x, u.y, u.z, u.w};
+    return kNorm ? double(v[j]) * double(f[j]) : double(v[j]);
+  };
   double ss = 0.0;
-  float m32 = 0.f;
+  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < E; i++) {
-    const float4 wf = widen(w[i]);
-    const float v[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, u[4] = {wf.x, wf.y, wf.z, wf.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (kNorm) {
-        const double d = double(v[j]);
-        ss = fma(d, d, ss);
-      }
-      const float p = fabsf(kNorm ? __fmul_rn(v[j], u[j]) : v[j]);
-      m32 = p <= m32 ? m32 : p;  // a NaN stays
+    const int at = 4 * (tid + i * blockDim.x), left = a.cols - at;
+    if constexpr (SRC == kRowAddNorm) {
+      h[i] = make_float4(__fadd_rn(h[i].x, y[i].x), __fadd_rn(h[i].y, y[i].y), __fadd_rn(h[i].z, y[i].z),
+                         __fadd_rn(h[i].w, y[i].w));
+      if (left > 0) store4<VEC>(const_cast<float*>(xf) + at, left, h[i]);
     }
-  }
-  unsigned long long amax = 0;
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    const float4 wf = widen(w[i]);
-    const float v[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, u[4] = {wf.x, wf.y, wf.z, wf.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float p = fabsf(kNorm ? __fmul_rn(v[j], u[j]) : v[j]);
-      if (!(p < m32)) amax = max(amax, abs_bits(kNorm ? double(v[j]) * double(u[j]) : double(v[j])));
+    if constexpr (kNorm) {
+      const double d0 = h[i].x, d1 = h[i].y, d2 = h[i].z, d3 = h[i].w;
+      ss = fma(d0, d0, ss), ss = fma(d1, d1, ss), ss = fma(d2, d2, ss), ss = fma(d3, d3, ss);
     }
+    float p[4];
+    products(i, p);
+    m = max_abs(p[3], max_abs(p[2], max_abs(p[1], max_abs(p[0], m))));
   }
+  unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(m));  // as integers: NaN above infinity
+  if (kNorm) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if (kNorm) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   }
   if (warps > 1) {  // one row a block
-    if ((tid & 31) == 0) {
+    if (lane == 0) {
       red_s[tid >> 5] = ss;
-      red_m[tid >> 5] = amax;
+      red_m[tid >> 5] = top;
     }
     __syncthreads();
-    const int l = tid & 31;
-    ss = l < warps ? red_s[l] : 0.0;
-    amax = l < warps ? red_m[l] : 0ull;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (kNorm) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? red_m[lane] : 0u);
+    if (kNorm) {
+      // Each group of `span` lanes (a power of two, at least the number of warps) adds the warps' sums.
+      const int span = 1 << (32 - __clz(warps - 1));
+      ss = (lane & (span - 1)) < warps ? red_s[lane & (span - 1)] : 0.0;
+      for (int o = span / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     }
   }
-  const double r = kNorm ? 1.0 / sqrt(ss / double(a.cols) + a.eps) : 1.0;
-  float s;
-  const RowScale k = row_scale(amax, r, &s);
-  if (tid == 0) a.scale[row] = s;
+  double amax = double(__uint_as_float(top));
+  if (kNorm) {
+    // Exactly, of the products that round to the largest.
+    unsigned long long best = 0;
+    if (__float_as_uint(m) == top) {
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        float p[4];
+        products(i, p);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (fabsf(p[j]) == m) best = max(best, abs_bits(value(i, j)));
+      }
+    }
+    if (warps > 1) {
+      if (best) atomicMax(&exact, best);
+      __syncthreads();
+      best = exact;
+    } else {
+      best = warp_max64(best);
+    }
+    if (!isnan(__uint_as_float(top))) amax = __longlong_as_double(static_cast<long long>(best));
+  }
+  const RowScale k = row_scale(amax, kNorm ? rsqrt(fma(ss, a.inv_cols, a.eps)) : 1.0);
+  if (tid == 0) a.scale[row] = k.s;
   int8_t* q = a.q + row * a.ld;
 #pragma unroll
   for (int i = 0; i < E; i++) {
     const int at = 4 * (tid + i * blockDim.x);
     if (at >= a.ld) continue;  // the padding gets its zeros: values past the row's end are 0
-    const float4 wf = widen(w[i]);
-    const float v[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, u[4] = {wf.x, wf.y, wf.z, wf.w};
+    float p[4];
+    products(i, p);
     uint32_t b[4];
-    bool sure = k.fast;
+    float off = 0.f;  // the largest distance from an integer
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float d = __fmul_rn(kNorm ? __fmul_rn(v[j], u[j]) : v[j], k.c32);
+      const float d = __fmul_rn(p[j], k.c32);
       const float t = __fadd_rn(d, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are the rounded integer
       b[j] = __float_as_uint(t);
-      sure = sure && fabsf(__fsub_rn(d, __fsub_rn(t, 12582912.0f))) < 0.4999f;
+      off = max_abs(__fsub_rn(d, __fsub_rn(t, 12582912.0f)), off);
     }
-    if (!sure && !k.zero) {
+    if (!(off < k.sure)) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) b[j] = uint32_t(row_int(kNorm ? double(v[j]) * double(u[j]) : double(v[j]), k));
+      for (int j = 0; j < 4; j++) b[j] = uint32_t(row_int(value(i, j), k));
     }
-    uint32_t word = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    if (k.zero) word = 0;
-    *reinterpret_cast<uint32_t*>(q + at) = word;
+    *reinterpret_cast<uint32_t*>(q + at) =
+        __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
 }
 
@@ -270,10 +306,9 @@ __global__ void __launch_bounds__(1024) k_long_rows_q8(RowArgs a) {
     ss += red_s[i];
     amax = max(amax, red_m[i]);
   }
-  const double r = kNorm ? 1.0 / sqrt(ss / double(a.cols) + a.eps) : 1.0;
-  float s;
-  const RowScale k = row_scale(amax, r, &s);
-  if (threadIdx.x == 0) a.scale[row] = s;
+  const double r = kNorm ? rsqrt(fma(ss, a.inv_cols, a.eps)) : 1.0;
+  const RowScale k = row_scale(__longlong_as_double(static_cast<long long>(amax)), r);
+  if (threadIdx.x == 0) a.scale[row] = k.s;
   int8_t* q = a.q + row * a.ld;
   for (int i = threadIdx.x; i < a.ld; i += blockDim.x) {
     double v = 0.0;
@@ -281,44 +316,73 @@ __global__ void __launch_bounds__(1024) k_long_rows_q8(RowArgs a) {
       v = SRC == kRowBf16 ? double(bf16f(xh[i])) : double(xf[i]);
       if (kNorm) v *= double(bf16f(a.w[i]));
     }
-    q[i] = int8_t(row_int(v, k));
+    q[i] = int8_t(row_int(v, r, k.s));
   }
 }
 
-// Four values a thread; blockDim.x threads along a row, blockDim.y rows.
-template <bool VEC>
+// Groups of four values (the aligned ones of the output, whose
+// rows begin `shift` values after one where `cols` is no multiple of four: an
+// unaligned store4 each took 5000 x 2562 from 10.7 to 22 us), kDeq of them
+// a thread, so that a thread has more than one word on its way; blockDim.x
+// threads along a row, blockDim.y rows.
+constexpr int kDeq = 4;
 __global__ void __launch_bounds__(256) k_dequantize(float* __restrict__ out, const int8_t* __restrict__ q,
                                                     const float* __restrict__ scale, long long rows, int cols, int ld) {
   pdl_launch_dependents();
   pdl_wait();
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= rows) return;
-  const float s = scale[row];
-  for (int at = 4 * (threadIdx.x + blockIdx.y * blockDim.x); at < cols; at += 4 * blockDim.x * gridDim.y) {
-    const char4 v = *reinterpret_cast<const char4*>(q + row * ld + at);
-    store4<VEC>(out + row * cols + at, cols - at,
-                make_float4(__fmul_rn(float(v.x), s), __fmul_rn(float(v.y), s), __fmul_rn(float(v.z), s),
-                            __fmul_rn(float(v.w), s)));
+  const int shift = int((row * cols) & 3), groups = (cols + shift + 3) / 4;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(q + row * ld);
+  float* to = out + row * cols;
+  for (int g0 = threadIdx.x + kDeq * blockDim.x * blockIdx.y; g0 < groups; g0 += kDeq * blockDim.x * gridDim.y) {
+    uint32_t v[kDeq];
+#pragma unroll
+    for (int i = 0; i < kDeq; i++) {
+      const int g = g0 + i * blockDim.x;
+      if (g >= groups) continue;
+      v[i] = 4 * g < ld ? words[g] : 0;
+      if (shift) v[i] = __funnelshift_l(g ? words[g - 1] : 0, v[i], 8 * shift);
+    }
+    const float s = scale[row];
+#pragma unroll
+    for (int i = 0; i < kDeq; i++) {
+      const int g = g0 + i * blockDim.x, at = 4 * g - shift;
+      if (g >= groups) continue;
+      const float4 x = make_float4(float(int8_t(v[i])), float(int8_t(v[i] >> 8)), float(int8_t(v[i] >> 16)),
+                                   float(int8_t(v[i] >> 24)));
+      const float4 y = make_float4(__fmul_rn(x.x, s), __fmul_rn(x.y, s), __fmul_rn(x.z, s), __fmul_rn(x.w, s));
+      if (at >= 0 && at + 4 <= cols) {
+        *reinterpret_cast<float4*>(to + at) = y;
+      } else {
+        const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (at + j >= 0 && at + j < cols) to[at + j] = e[j];
+      }
+    }
   }
 }
 
 template <int SRC>
 void launch_rows_q8(tb200_device* d, const RowArgs& a, size_t rows) {
-  // Threads that have four values each; the padding (fewer than 16) is theirs too.
-  const int groups = a.ld / 4;
-  const bool vec = a.cols % 4 == 0;
-  // Few rows: as many threads on each as it has groups, since what counts is
-  // how long one row takes. Many: several groups a thread, so that more of a
-  // row's loads are in flight at once and its reduction is shared by fewer warps.
-  const bool few = rows < size_t(2 * d->sms);
+  constexpr bool kNorm = SRC == kRowNorm || SRC == kRowAddNorm;
+  const int groups = a.ld / 4;  // of four values; the padding is theirs too
+  // Few rows: as many threads on each as it has groups, since what counts is how
+  // long one row takes. Many: as few warps as can hold it, one if it fits, up to
+  // four groups a thread with a norm, eight without (2048 x 9728: 31 and 17 us with
+  // four and eight; with the residual and the norm 54 and 83, for want of registers).
   int e = 1;
-  while (e < 4 && groups > e * (few ? 1024 : 128)) e *= 2;
-  if (groups > e * 1024) {
+  if (rows >= size_t(2 * d->sms))
+    while (e < (kNorm ? 4 : 8) && groups > e * 32) e *= 2;
+  while (e < 8 && groups > e * row_threads(e)) e *= 2;
+  if (groups > e * row_threads(e)) {
     launch_pdl(k_long_rows_q8<SRC>, dim3(unsigned(rows)), dim3(1024), 0, d->stream, a);
     return;
   }
   const int tx = (groups + 32 * e - 1) / (32 * e) * 32, ty = tx == 32 ? 4 : 1;
   const dim3 grid(unsigned((rows + ty - 1) / ty)), block(tx, ty);
+  const bool vec = a.cols % 4 == 0;
 #define TB_ROWS(E)                                                                               \
   if (e == E) {                                                                                  \
     if (vec)                                                                                     \
@@ -329,6 +393,7 @@ void launch_rows_q8(tb200_device* d, const RowArgs& a, size_t rows) {
   TB_ROWS(1)
   TB_ROWS(2)
   TB_ROWS(4)
+  TB_ROWS(8)
 #undef TB_ROWS
 }
 
@@ -337,6 +402,7 @@ RowArgs row_args(const tb200_q8* out) {
   a.q = out->values;
   a.scale = out->scales;
   a.cols = int(out->cols);
+  a.inv_cols = 1.0 / double(out->cols);
   a.ld = int(out->ld);
   return a;
 }
@@ -470,17 +536,16 @@ int tb200_dequantize(tb200_device* d, tb200_buffer* out, const tb200_q8* x) {
   ARG_CHECK(out->len == x->rows * x->cols, "dequantize: output holds " + std::to_string(out->len) +
                                                " values, expected " + std::to_string(x->rows * x->cols));
   if (!x->rows) return TB200_OK;
-  const size_t groups = (x->cols + 3) / 4;
+  const size_t groups = (x->cols + (x->cols % 4 ? 3 : 0) + 3) / 4;
+  // Few rows: a group a thread, as many threads as there are; many: kDeq groups a thread.
+  const size_t each = x->rows * groups < size_t(d->sms) * 2048 ? 1 : tb::kDeq;
   unsigned tx = 32;
-  while (tx < 256 && tx < groups) tx *= 2;
+  while (tx < 256 && tx * each < groups) tx *= 2;
   const unsigned ty = 256 / tx;
-  const dim3 grid(unsigned((x->rows + ty - 1) / ty), unsigned(std::min<size_t>((groups + tx - 1) / tx, 65535)));
-  if (x->cols % 4 == 0)
-    tb::launch_pdl(tb::k_dequantize<true>, grid, dim3(tx, ty), 0, d->stream, out->ptr, x->values, x->scales,
-                   (long long)x->rows, int(x->cols), int(x->ld));
-  else
-    tb::launch_pdl(tb::k_dequantize<false>, grid, dim3(tx, ty), 0, d->stream, out->ptr, x->values, x->scales,
-                   (long long)x->rows, int(x->cols), int(x->ld));
+  const size_t along = (groups + tx * tb::kDeq - 1) / (tx * tb::kDeq);
+  const dim3 grid(unsigned((x->rows + ty - 1) / ty), unsigned(std::min<size_t>(along, 65535)));
+  tb::launch_pdl(tb::k_dequantize, grid, dim3(tx, ty), 0, d->stream, out->ptr, x->values, x->scales,
+                 (long long)x->rows, int(x->cols), int(x->ld));
   return rt::launched("dequantize");
 }
 
