@@ -40,38 +40,67 @@ namespace tb {
 namespace {
 constexpr size_t kMaxCols = 131071;  // 128 * 128 * 131071 < 2^31
 
-// One warp per channel and up to 4 tokens.
+// A warp per R channels and up to kVecTokens tokens: R rows' loads are on their
+// way at once.
+constexpr int kVecTokens = 4;
+template <int T, int R>
 __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, const int8_t* __restrict__ w,
                                                    const float* __restrict__ sw, int channels,
-                                                   const int8_t* __restrict__ x, const float* __restrict__ sx,
-                                                   int tokens, int ldw, int ldx) {
+                                                   const int8_t* __restrict__ x, const float* __restrict__ sx, int ldw,
+                                                   int ldx) {
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = blockIdx.x * 8 + warp, t0 = blockIdx.y * 4;
-  if (c >= channels) return;
-  int acc[4] = {0, 0, 0, 0};
-  const int4* wr = reinterpret_cast<const int4*>(w + size_t(c) * ldw);
-  for (int i = lane; i < ldw / 16; i += 32) {
-    const int4 a = wr[i];
+  const int c0 = (blockIdx.x * 8 + warp) * R;
+  if (c0 >= channels) return;
+  int acc[R][T];
+  const int4* wr[R];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      if (t0 + t >= tokens) break;
-      const int4 b = reinterpret_cast<const int4*>(x + size_t(t0 + t) * ldx)[i];
-      acc[t] = __dp4a(a.x, b.x, acc[t]);
-      acc[t] = __dp4a(a.y, b.y, acc[t]);
-      acc[t] = __dp4a(a.z, b.z, acc[t]);
-      acc[t] = __dp4a(a.w, b.w, acc[t]);
+  for (int r = 0; r < R; r++) {
+    wr[r] = reinterpret_cast<const int4*>(w + size_t(min(c0 + r, channels - 1)) * ldw);
+#pragma unroll
+    for (int t = 0; t < T; t++) acc[r][t] = 0;
+  }
+  const int n = ldw / 16;
+#pragma unroll 2
+  for (int i = lane; i < n; i += 32) {
+    int4 a[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) a[r] = __ldcs(wr[r] + i);
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const int4 b = __ldg(reinterpret_cast<const int4*>(x + size_t(t) * ldx) + i);
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        acc[r][t] = __dp4a(a[r].x, b.x, acc[r][t]);
+        acc[r][t] = __dp4a(a[r].y, b.y, acc[r][t]);
+        acc[r][t] = __dp4a(a[r].z, b.z, acc[r][t]);
+        acc[r][t] = __dp4a(a[r].w, b.w, acc[r][t]);
+      }
     }
   }
+  int mine = 0;
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const int s = __reduce_add_sync(0xffffffffu, acc[t]);
-    if (lane == t && t0 + t < tokens)
-      out[size_t(t0 + t) * channels + c] = __fmul_rn(__int2float_rn(s), __fmul_rn(sw[c], sx[t0 + t]));
-  }
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const int s = __reduce_add_sync(0xffffffffu, acc[r][t]);
+      if (lane == t * R + r) mine = s;
+    }
+  const int c = c0 + lane % R, t = lane / R;
+  if (t < T && c < channels)
+    out[size_t(t) * channels + c] = __fmul_rn(__int2float_rn(mine), __fmul_rn(sw[c], sx[t]));
 }
 
+template <int T>
+void matvec_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
+  const int channels = int(w->rows);
+  auto go = [&](auto kernel, int r) {
+    launch_pdl(kernel, dim3(unsigned((channels + 8 * r - 1) / (8 * r))), dim3(256), 0, d->stream, out, w->values,
+               w->scales, channels, x->values, x->scales, int(w->ld), int(x->ld));
+  };
+  go(k_matvec_q8<T, T == 1 ? 1 : 2>, T == 1 ? 1 : 2);
+}
 
 // ---- tensor cores ------------------------------------------------------------
 
@@ -135,6 +164,16 @@ __device__ __forceinline__ void q_mma(uint32_t tmem_d, uint64_t a, uint64_t b, u
       "l"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
+// True for one lane of the (converged) warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void q_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -165,9 +204,12 @@ __global__ void __launch_bounds__(kQThreads, 1)
   QTail& tl = *reinterpret_cast<QTail*>(sm + q_ring_bytes(n, a.xrows, stages));
   auto sB = [&](int s) { return sm + size_t(s) * stage_bytes; };
   auto sA = [&](int s) { return sm + size_t(s) * stage_bytes + size_t(n) * kKB; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int nkb = (a.K + kKB - 1) / kKB;
   const int tiles = a.mtiles * a.ntiles;
+  // Each CTA begins its sums at another place of K: the order is free, and CTAs
+  // that share token rows do not all ask the same L2 slices for them at once.
+  const int k0 = int((long long)blockIdx.x * nkb / gridDim.x);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
@@ -187,6 +229,10 @@ __global__ void __launch_bounds__(kQThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (threadIdx.x == 32 * 2) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tw)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tx)) : "memory");
+  }
   q_fence_before();
   __syncthreads();
   q_fence_after();
@@ -194,58 +240,64 @@ __global__ void __launch_bounds__(kQThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
+  // The producer's and the MMA warp's lanes stay together and one of them is
+  // elected at each instruction: what they issue takes uniform registers, and
+  // in a branch of one lane the compiler has to move every operand there.
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
-      int i = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
-        for (int k = 0; k < nkb; k++, i++) {
-          const int s = i % stages;
-          if (!mbar_wait(&tl.empty[s], ((i / stages) & 1) ^ 1, a.err)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&tl.full[s], stage_bytes);
-          tma_load_2d(sB(s), &tw, k * kKB, n0, &tl.full[s], pol_w);
-          tma_load_2d(sA(s), &tx, k * kKB, m0, &tl.full[s], pol_x);
+    const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
+    int i = 0, s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
+      for (int k = 0; k < nkb; k++, i++) {
+        if (!mbar_wait(&tl.empty[s], phase, a.err)) {
+          ok = false;
+          break;
         }
+        const int at = (k + k0 < nkb ? k + k0 : k + k0 - nkb) * kKB;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&tl.full[s], stage_bytes);
+          tma_load_2d(sB(s), &tw, at, n0, &tl.full[s], pol_w);
+          tma_load_2d(sA(s), &tx, at, m0, &tl.full[s], pol_x);
+        }
+        if (++s == stages) s = 0, phase ^= 1;
       }
-      // Every issued copy has landed before the CTA can exit.
-      for (int j = i - 1; j >= 0 && j >= i - stages; j--) mbar_wait(&tl.full[j % stages], (j / stages) & 1, nullptr);
     }
+    // Every issued copy has landed before the CTA can exit.
+    for (int j = i - 1; j >= 0 && j >= i - stages; j--) mbar_wait(&tl.full[j % stages], (j / stages) & 1, nullptr);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = q_idesc(kTileM, n);
-      int i = 0, ti = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ti++) {
-        const int b = ti & 1;
-        // The epilogue has drained this accumulator's previous tile.
-        if (!mbar_wait(&tl.tempty[b], ((ti >> 1) - 1) & 1, a.err)) break;
+    const uint32_t idesc = q_idesc(kTileM, n);
+    const uint64_t desc0 = q_desc(smem_u32(sm));
+    int s = 0, ti = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ti++) {
+      const int b = ti & 1;
+      // The epilogue has drained this accumulator's previous tile.
+      if (!mbar_wait(&tl.tempty[b], ((ti >> 1) - 1) & 1, a.err)) break;
+      q_fence_after();
+      const uint32_t acc = tmem + uint32_t(b * kMaxN);
+      for (int k = 0; k < nkb; k++) {
+        if (!mbar_wait(&tl.full[s], phase, a.err)) {
+          ok = false;
+          break;
+        }
         q_fence_after();
-        const uint32_t acc = tmem + uint32_t(b * kMaxN);
-        for (int k = 0; k < nkb; k++, i++) {
-          const int s = i % stages;
-          if (!mbar_wait(&tl.full[s], (i / stages) & 1, a.err)) {
-            ok = false;
-            break;
-          }
-          q_fence_after();
-          const uint32_t a0 = smem_u32(sA(s)), b0 = smem_u32(sB(s));
+        const uint64_t db = desc0 + ((s * stage_bytes) >> 4), da = db + ((uint32_t(n) * kKB) >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kKB / 32; kk++)
-            q_mma(acc, q_desc(a0 + 32 * kk), q_desc(b0 + 32 * kk), idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            q_mma(acc, da + 2 * kk, db + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
           q_commit(&tl.empty[s]);
         }
-        if (ok) q_commit(&tl.tfull[b]);
+        if (++s == stages) s = 0, phase ^= 1;
       }
-      // Tensor memory is freed below only after every MMA has completed.
-      q_commit(&tl.mdone);
-      mbar_wait(&tl.mdone, 0, nullptr);
+      if (ok && elect_one()) q_commit(&tl.tfull[b]);
     }
-    __syncwarp();
+    // Tensor memory is freed below only after every MMA has completed.
+    if (elect_one()) q_commit(&tl.mdone);
+    mbar_wait(&tl.mdone, 0, nullptr);
   } else {
     const int q = warp & 3;  // the 32 accumulator lanes this warp can read
     const int e = int(threadIdx.x) - 64;
@@ -388,10 +440,13 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   ARG_CHECK(out->len == x->rows * w->rows, "matmul_q8: output holds " + std::to_string(out->len) + ", expected " +
                                                std::to_string(x->rows * w->rows));
   if (!x->rows || !w->rows) return TB200_OK;
-  if (x->rows > 4) return tb::gemm_q8(d, out->ptr, w, x);
-  const dim3 grid(unsigned((w->rows + 7) / 8), unsigned((x->rows + 3) / 4));
-  tb::launch_pdl(tb::k_matvec_q8, grid, dim3(256), 0, d->stream, out->ptr, w->values, w->scales, int(w->rows),
-                 x->values, x->scales, int(x->rows), int(w->ld), int(x->ld));
+  switch (getenv("TBG") ? 99 : x->rows) {
+    case 1: tb::matvec_q8<1>(d, out->ptr, w, x); break;
+    case 2: tb::matvec_q8<2>(d, out->ptr, w, x); break;
+    case 3: tb::matvec_q8<3>(d, out->ptr, w, x); break;
+    case 4: tb::matvec_q8<4>(d, out->ptr, w, x); break;
+    default: return tb::gemm_q8(d, out->ptr, w, x);
+  }
   return rt::launched("matmul_q8");
 }
 
