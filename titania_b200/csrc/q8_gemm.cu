@@ -156,13 +156,22 @@ __device__ __forceinline__ uint64_t q_desc(uint32_t saddr) {
 __device__ __forceinline__ uint32_t q_idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
+template <int CG>
 __device__ __forceinline__ void q_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accum)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum)
+        : "memory");
 }
 // True for one lane of the (converged) warp, the same each time.
 __device__ __forceinline__ bool elect_one() {
@@ -174,9 +183,61 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(p));
   return p != 0;
 }
+// Arrives on `bar` (with a pair: on both CTAs' barrier at that place) once
+// every MMA issued so far has completed.
+template <int CG>
 __device__ __forceinline__ void q_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(uint16_t(3))
+        : "memory");
+}
+// tma_load_2d into this CTA, completing on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(void* dst, const void* map, int x, int y, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address, as the pair's CTAs see it, of a shared variable in its first CTA.
+__device__ __forceinline__ uint32_t in_first(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+// mbar_wait for arrivals from the other CTA of the pair.
+__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, int* err) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitCycles) {
+      set_error(err, TB200_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 16 consecutive 32-bit columns of this warp's 32 lanes.
 __device__ __forceinline__ void q_tmem_ld16(uint32_t addr, int (&r)[16]) {
@@ -194,22 +255,29 @@ __device__ __forceinline__ void st8(float* p, const float* v) {
                : "memory");
 }
 
+// CG CTAs work on a tile of 128 CG tokens by n channels. A pair (CG = 2) sits
+// on neighbouring SMs: each CTA loads its 128 tokens and half of the channels,
+// the first one's MMA warp issues MMAs of 256 tokens over both CTAs' shared
+// memory, and each CTA finds its tokens' sums in its own tensor memory. Per
+// output that takes two thirds of one CTA's bytes from L2, which is what
+// bounds many tokens.
+template <int CG>
 __global__ void __launch_bounds__(kQThreads, 1)
     k_gemm_q8(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, QGemmArgs a) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles: 1024-byte alignment
-  const int stages = a.stages, n = a.n;
-  const uint32_t stage_bytes = uint32_t(q_stage_bytes(n, a.xrows));
-  QTail& tl = *reinterpret_cast<QTail*>(sm + q_ring_bytes(n, a.xrows, stages));
-  auto sB = [&](int s) { return sm + size_t(s) * stage_bytes; };
-  auto sA = [&](int s) { return sm + size_t(s) * stage_bytes + size_t(n) * kKB; };
+  const int stages = a.stages, n = a.n, wrows = n / CG;
+  const uint32_t stage_bytes = uint32_t(q_stage_bytes(wrows, a.xrows));
+  QTail& tl = *reinterpret_cast<QTail*>(sm + q_ring_bytes(wrows, a.xrows, stages));
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? int(pair_rank()) : 0;
+  const int group = int(blockIdx.x) / CG, groups = int(gridDim.x) / CG;
   const int nkb = (a.K + kKB - 1) / kKB;
   const int tiles = a.mtiles * a.ntiles;
-  // Each CTA begins its sums at another place of K: the order is free, and CTAs
-  // that share token rows do not all ask the same L2 slices for them at once.
-  const int k0 = int((long long)blockIdx.x * nkb / gridDim.x);
+  // Each group begins its sums at another place of K: the order is free, and
+  // CTAs that share token rows do not all ask the same L2 slices for them at once.
+  const int k0 = int((long long)group * nkb / groups);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
@@ -218,16 +286,23 @@ __global__ void __launch_bounds__(kQThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tl.tfull[b], 1);
-      mbar_init(&tl.tempty[b], 4);  // one arrival per epilogue warp
+      mbar_init(&tl.tempty[b], 4 * CG);  // one arrival per epilogue warp
     }
     mbar_init(&tl.mdone, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tl.tmem)),
-                 "r"(kQTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tl.tmem)),
+                   "r"(kQTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tl.tmem)),
+                   "r"(kQTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   if (threadIdx.x == 32 * 2) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tw)) : "memory");
@@ -235,6 +310,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
   }
   q_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) pair_sync();  // both CTAs' barriers and tensor memory are there
   q_fence_after();
   const uint32_t tmem = tl.tmem;
   pdl_launch_dependents();
@@ -242,69 +318,84 @@ __global__ void __launch_bounds__(kQThreads, 1)
 
   // The producer's and the MMA warp's lanes stay together and one of them is
   // elected at each instruction: what they issue takes uniform registers, and
-  // in a branch of one lane the compiler has to move every operand there.
+  // in a branch of one lane the compiler has to move every operand there
+  // (64 x 19456 x 2560: 10.9 us instead of 7.3).
   if (warp == 0) {
     const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
     int i = 0, s = 0;
     uint32_t phase = 1;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
+    for (int tile = group; tile < tiles && ok; tile += groups) {
+      const int m0 = (tile % a.mtiles * CG + rank) * kTileM, n0 = tile / a.mtiles * n + rank * wrows;
       for (int k = 0; k < nkb; k++, i++) {
         if (!mbar_wait(&tl.empty[s], phase, a.err)) {
           ok = false;
           break;
         }
         const int at = (k + k0 < nkb ? k + k0 : k + k0 - nkb) * kKB;
+        unsigned char *dw = sm + size_t(s) * stage_bytes, *dx = dw + size_t(wrows) * kKB;
         if (elect_one()) {
-          mbar_arrive_expect_tx(&tl.full[s], stage_bytes);
-          tma_load_2d(sB(s), &tw, at, n0, &tl.full[s], pol_w);
-          tma_load_2d(sA(s), &tx, at, m0, &tl.full[s], pol_x);
+          // The first CTA's barrier counts both CTAs' bytes, of which the second's may come before it
+          // expects them.
+          if (rank == 0) mbar_arrive_expect_tx(&tl.full[s], CG * stage_bytes);
+          if constexpr (CG == 1) {
+            tma_load_2d(dw, &tw, at, n0, &tl.full[s], pol_w);
+            tma_load_2d(dx, &tx, at, m0, &tl.full[s], pol_x);
+          } else {
+            const uint32_t bar = in_first(&tl.full[s]);
+            tma_load_pair(dw, &tw, at, n0, bar, pol_w);
+            tma_load_pair(dx, &tx, at, m0, bar, pol_x);
+          }
         }
         if (++s == stages) s = 0, phase ^= 1;
       }
     }
-    // Every issued copy has landed before the CTA can exit.
-    for (int j = i - 1; j >= 0 && j >= i - stages; j--) mbar_wait(&tl.full[j % stages], (j / stages) & 1, nullptr);
+    // Every issued copy has landed before the CTA can exit: it has been waited
+    // for, or (the second CTA's) read.
+    for (int j = i - 1; j >= 0 && j >= i - stages; j--)
+      mbar_wait(rank == 0 ? &tl.full[j % stages] : &tl.empty[j % stages], (j / stages) & 1, nullptr);
   } else if (warp == 1) {
-    const uint32_t idesc = q_idesc(kTileM, n);
-    const uint64_t desc0 = q_desc(smem_u32(sm));
-    int s = 0, ti = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ti++) {
-      const int b = ti & 1;
-      // The epilogue has drained this accumulator's previous tile.
-      if (!mbar_wait(&tl.tempty[b], ((ti >> 1) - 1) & 1, a.err)) break;
-      q_fence_after();
-      const uint32_t acc = tmem + uint32_t(b * kMaxN);
-      for (int k = 0; k < nkb; k++) {
-        if (!mbar_wait(&tl.full[s], phase, a.err)) {
-          ok = false;
-          break;
-        }
+    if (rank == 0) {
+      const uint32_t idesc = q_idesc(CG * kTileM, n);
+      const uint64_t desc0 = q_desc(smem_u32(sm));
+      int s = 0, ti = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = group; tile < tiles && ok; tile += groups, ti++) {
+        const int b = ti & 1;
+        // The epilogue has drained this accumulator's previous tile.
+        const uint32_t drained = ((ti >> 1) - 1) & 1;
+        if (!(CG == 1 ? mbar_wait(&tl.tempty[b], drained, a.err) : pair_wait(&tl.tempty[b], drained, a.err))) break;
         q_fence_after();
-        const uint64_t db = desc0 + ((s * stage_bytes) >> 4), da = db + ((uint32_t(n) * kKB) >> 4);
-        if (elect_one()) {
+        const uint32_t acc = tmem + uint32_t(b * kMaxN);
+        for (int k = 0; k < nkb; k++) {
+          if (!mbar_wait(&tl.full[s], phase, a.err)) {
+            ok = false;
+            break;
+          }
+          q_fence_after();
+          const uint64_t db = desc0 + ((s * stage_bytes) >> 4), da = db + ((uint32_t(wrows) * kKB) >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKB / 32; kk++)
-            q_mma(acc, da + 2 * kk, db + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
-          q_commit(&tl.empty[s]);
+            for (int kk = 0; kk < kKB / 32; kk++)
+              q_mma<CG>(acc, da + 2 * kk, db + 2 * kk, idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            q_commit<CG>(&tl.empty[s]);
+          }
+          if (++s == stages) s = 0, phase ^= 1;
         }
-        if (++s == stages) s = 0, phase ^= 1;
+        if (ok && elect_one()) q_commit<CG>(&tl.tfull[b]);
       }
-      if (ok && elect_one()) q_commit(&tl.tfull[b]);
+      // Tensor memory is freed below only after every MMA has completed.
+      if (elect_one()) q_commit<CG>(&tl.mdone);
+      mbar_wait(&tl.mdone, 0, nullptr);
     }
-    // Tensor memory is freed below only after every MMA has completed.
-    if (elect_one()) q_commit(&tl.mdone);
-    mbar_wait(&tl.mdone, 0, nullptr);
   } else {
     const int q = warp & 3;  // the 32 accumulator lanes this warp can read
     const int e = int(threadIdx.x) - 64;
     int ti = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ti++) {
+    for (int tile = group; tile < tiles; tile += groups, ti++) {
       const int b = ti & 1;
-      const int m0 = tile % a.mtiles * kTileM, n0 = tile / a.mtiles * n;
+      const int m0 = (tile % a.mtiles * CG + rank) * kTileM, n0 = tile / a.mtiles * n;
       const int cols = min(n, a.M - n0);
       for (int j = e; j < n; j += 128) tl.sw[b][j] = j < cols ? a.sw[n0 + j] : 0.f;
       const int t = m0 + 32 * q + lane;
@@ -346,14 +437,24 @@ __global__ void __launch_bounds__(kQThreads, 1)
       }
       q_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tl.tempty[b]);
+      if (lane == 0) {
+        if constexpr (CG == 1)
+          mbar_arrive(&tl.tempty[b]);
+        else
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(&tl.tempty[b]))
+                       : "memory");
+      }
     }
   }
   q_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) pair_sync();  // no MMA reads the other CTA's memory, no arrival is on its way there
   if (warp == 1) {
     q_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kQTmemCols) : "memory");
+    if constexpr (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kQTmemCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kQTmemCols) : "memory");
   }
 }
 
@@ -380,20 +481,21 @@ int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
   return TB200_OK;
 }
 
-// Channels per tile: the multiple of 16 with which the CTA that has most to do
-// has least, a tile's fixed cost (filling the ring, the last tile's epilogue)
-// counted as 24 channels.
-int plan_n(int M, int mtiles, int sms) {
+// Channels per tile: the multiple of `step` with which the group that has most
+// to do has least, a tile's fixed cost (filling the ring, the last tile's
+// epilogue) counted as 24 channels.
+int plan_n(int M, int mtiles, int groups, int step) {
   int best = 0;
   long long least = 0;
-  for (int n = 16; n <= kMaxN; n += 16) {
+  for (int n = step; n <= kMaxN; n += step) {
     const long long tiles = (long long)mtiles * ((M + n - 1) / n);
-    const long long cost = (tiles + sms - 1) / sms * (n + 24);
+    const long long cost = (tiles + groups - 1) / groups * (n + 24);
     if (!best || cost <= least) best = n, least = cost;
   }
   return best;
 }
 
+template <int CG>
 int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   QGemmArgs a{};
   a.sw = w->scales;
@@ -403,28 +505,42 @@ int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   a.M = int(w->rows);
   a.K = int(w->cols);
   a.err = d->async_err_dev;
-  a.mtiles = (a.T + kTileM - 1) / kTileM;
-  a.n = plan_n(a.M, a.mtiles, d->sms);
+  a.mtiles = (a.T + CG * kTileM - 1) / (CG * kTileM);
+  a.n = plan_n(a.M, a.mtiles, d->sms / CG, 16 * CG);
   a.ntiles = (a.M + a.n - 1) / a.n;
-  a.xrows = std::min(kTileM, (a.T + 7) / 8 * 8);
+  a.xrows = CG == 2 ? kTileM : std::min(kTileM, (a.T + 7) / 8 * 8);
+  const int wrows = a.n / CG;
   const size_t fixed = size_t(kTileM - a.xrows) * kKB + sizeof(QTail) + 1024;
-  a.stages = int(std::min<size_t>(kQMaxStages, (kQMaxSmem - fixed) / q_stage_bytes(a.n, a.xrows)));
+  a.stages = int(std::min<size_t>(kQMaxStages, (kQMaxSmem - fixed) / q_stage_bytes(wrows, a.xrows)));
   const uintptr_t al = reinterpret_cast<uintptr_t>(out) | (uintptr_t(a.M) * 4);
   a.vec = al % 32 == 0 ? 8 : al % 16 == 0 ? 4 : 1;
   CUtensorMap tw, tx;
-  if (int rc = encode_tmap_q8(&tw, w, a.n)) return rc;
+  if (int rc = encode_tmap_q8(&tw, w, wrows)) return rc;
   if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
-  const size_t smem =
-      std::max(kQMinSmem, q_ring_bytes(a.n, a.xrows, a.stages) + sizeof(QTail) + 1024);
-  const unsigned grid = unsigned(std::min<long long>((long long)a.mtiles * a.ntiles, d->sms));
-  launch_pdl(k_gemm_q8, dim3(grid), dim3(kQThreads), smem, d->stream, tw, tx, a);
+  const size_t smem = std::max(kQMinSmem, q_ring_bytes(wrows, a.xrows, a.stages) + sizeof(QTail) + 1024);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(CG * std::min<long long>((long long)a.mtiles * a.ntiles, d->sms / CG)));
+  cfg.blockDim = dim3(kQThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = d->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {CG, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = CG;  // one CTA: no cluster
+  cudaLaunchKernelEx(&cfg, k_gemm_q8<CG>, tw, tx, a);
   return rt::launched("matmul_q8");
 }
 
 }  // namespace
 
 cudaError_t init_q8_kernels() {
-  return cudaFuncSetAttribute(k_gemm_q8, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
+  cudaError_t e = cudaFuncSetAttribute(k_gemm_q8<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(k_gemm_q8<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
+  return e;
 }
 
 }  // namespace tb
@@ -440,12 +556,12 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   ARG_CHECK(out->len == x->rows * w->rows, "matmul_q8: output holds " + std::to_string(out->len) + ", expected " +
                                                std::to_string(x->rows * w->rows));
   if (!x->rows || !w->rows) return TB200_OK;
-  switch (getenv("TBG") ? 99 : x->rows) {
+  switch (x->rows) {
     case 1: tb::matvec_q8<1>(d, out->ptr, w, x); break;
     case 2: tb::matvec_q8<2>(d, out->ptr, w, x); break;
     case 3: tb::matvec_q8<3>(d, out->ptr, w, x); break;
     case 4: tb::matvec_q8<4>(d, out->ptr, w, x); break;
-    default: return tb::gemm_q8(d, out->ptr, w, x);
+    default: return x->rows > 128 && !getenv("TB1") ? tb::gemm_q8<2>(d, out->ptr, w, x) : tb::gemm_q8<1>(d, out->ptr, w, x);
   }
   return rt::launched("matmul_q8");
 }
