@@ -16,8 +16,11 @@
 //              and one of N channel rows (128-byte swizzle) into a ring;
 //   warp 1     one lane issues the MMAs (K = 32 each), commits each stage back
 //              to the producer and each tile to the epilogue;
-//   warps 2-5  epilogue: tcgen05.ld, scales, stores; two accumulators let it
-//              run behind the next tile's MMAs.
+//   warps 2-9  epilogue, two for each 32 lanes of the accumulator: tcgen05.ld, scales, then 32 x 32 outputs at a time
+//              through shared memory (128-byte swizzle) into a TMA store; two
+//              accumulators let it run behind the next tile's MMAs. With 32-byte
+//              stores from each lane's own row it took 450 to 790 cycles for 16
+//              columns, longer than the MMAs of a tile up to K = 2560.
 // Persistent CTAs walk the tiles, token tiles innermost, so that a channel
 // tile comes from memory once. Only the token rows that exist are loaded: the
 // MMA reads whatever shared memory holds in the place of the others, and the
@@ -107,7 +110,8 @@ void matvec_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x
 constexpr int kTileM = 128;              // token rows per CTA
 constexpr int kMaxN = 256;               // channels per tile
 constexpr int kKB = 128;                 // K per stage: one 128-byte swizzle row
-constexpr int kQThreads = 192;
+constexpr int kQThreads = 320;
+constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
 constexpr int kQTmemCols = 512;          // two accumulators of up to 256 columns
 constexpr int kQMaxStages = 24;
 constexpr size_t kQMinSmem = 116 * 1024;  // more than half of an SM's 228 KB
@@ -121,23 +125,28 @@ struct QGemmArgs {
   int n;             // channels per tile
   int xrows;         // token rows per tile that are loaded (a multiple of 8, at most 128)
   int stages, mtiles, ntiles;
-  int vec;           // floats per store that the output rows' alignment allows: 8, 4 or 1
+  int tma_out;       // output rows begin on 16-byte boundaries: a TMA store can write them
   int* err;
 };
 
-// Shared memory after the ring: barriers full[s], empty[s], tfull[2], tempty[2],
+// The epilogue's staging: a tile of 32 tokens by 32 channels for each warp.
+constexpr int kStageTile = 32 * 128;
+constexpr size_t kStaging = size_t(kEpiWarps) * kStageTile;
+
+// Shared memory after the ring and the staging: barriers full[s], empty[s], tfull[2], tempty[2],
 // mdone, then the address of the tensor memory and the epilogue's scales.
 struct QTail {
   uint64_t full[kQMaxStages], empty[kQMaxStages], tfull[2], tempty[2], mdone;
   uint32_t tmem;
-  int ok[4];
+  int ok[kEpiWarps];
   alignas(16) float sw[2][kMaxN];
 };
 
 __host__ __device__ constexpr size_t q_stage_bytes(int n, int xrows) { return size_t(n + xrows) * kKB; }
-// The last stage's MMA reads 128 token rows whatever xrows is.
+// The last stage's MMA reads 128 token rows whatever xrows is: into the staging.
+static_assert(kStaging >= size_t(kTileM) * kKB, "those reads stay inside shared memory");
 __host__ __device__ constexpr size_t q_ring_bytes(int n, int xrows, int stages) {
-  return stages * q_stage_bytes(n, xrows) + size_t(kTileM - xrows) * kKB;
+  return stages * q_stage_bytes(n, xrows);
 }
 
 __device__ __forceinline__ void q_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -239,19 +248,28 @@ __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// 16 consecutive 32-bit columns of this warp's 32 lanes.
-__device__ __forceinline__ void q_tmem_ld16(uint32_t addr, int (&r)[16]) {
+// 32 consecutive 32-bit columns of this warp's 32 lanes.
+__device__ __forceinline__ void q_tmem_ld32(uint32_t addr, int (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// Eight floats to a 32-byte aligned address in one store (a whole sector).
-__device__ __forceinline__ void st8(float* p, const float* v) {
-  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
-               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+// Waits for this warp's loads from tensor memory; `r` is not read before.
+__device__ __forceinline__ void q_tmem_wait(int (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+}
+// Stores a box from shared memory at (x, y); its elements outside the map are left out.
+__device__ __forceinline__ void tma_store_2d(const void* map, int x, int y, const void* src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
                : "memory");
 }
 
@@ -263,13 +281,15 @@ __device__ __forceinline__ void st8(float* p, const float* v) {
 // bounds many tokens.
 template <int CG>
 __global__ void __launch_bounds__(kQThreads, 1)
-    k_gemm_q8(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, QGemmArgs a) {
+    k_gemm_q8(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+              const __grid_constant__ CUtensorMap tout, const __grid_constant__ CUtensorMap tout16, QGemmArgs a) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles: 1024-byte alignment
   const int stages = a.stages, n = a.n, wrows = n / CG;
   const uint32_t stage_bytes = uint32_t(q_stage_bytes(wrows, a.xrows));
-  QTail& tl = *reinterpret_cast<QTail*>(sm + q_ring_bytes(wrows, a.xrows, stages));
+  unsigned char* staging = sm + q_ring_bytes(wrows, a.xrows, stages);
+  QTail& tl = *reinterpret_cast<QTail*>(staging + kStaging);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = CG == 2 ? int(pair_rank()) : 0;
   const int group = int(blockIdx.x) / CG, groups = int(gridDim.x) / CG;
@@ -286,7 +306,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tl.tfull[b], 1);
-      mbar_init(&tl.tempty[b], 4 * CG);  // one arrival per epilogue warp
+      mbar_init(&tl.tempty[b], kEpiWarps * CG);  // one arrival per epilogue warp
     }
     mbar_init(&tl.mdone, 1);
     fence_mbar_init();
@@ -393,46 +413,83 @@ __global__ void __launch_bounds__(kQThreads, 1)
     const int q = warp & 3;  // the 32 accumulator lanes this warp can read
     const int e = int(threadIdx.x) - 64;
     int ti = 0;
+    // This lane's row of the warp's staging tile: 16-byte piece j lies at j ^ (row & 7).
+    unsigned char* tile_s = staging + (warp - 2) * kStageTile;
+    float4* mine_s = reinterpret_cast<float4*>(tile_s + lane * 128);
+    // The scales of a tile are fetched while the one before is written.
+    static_assert(kEpiThreads == kMaxN, "a channel's scale for each thread");
+    float next_sw = 0.f, next_sx = 0.f;
+    auto fetch = [&](int tile) {
+      if (tile >= tiles) return;
+      const int t = (tile % a.mtiles * CG + rank) * kTileM + 32 * q + lane, c = tile / a.mtiles * n + e;
+      next_sw = e < n && c < a.M ? a.sw[c] : 0.f;
+      next_sx = t < a.T ? a.sx[t] : 0.f;
+    };
+    fetch(group);
     for (int tile = group; tile < tiles; tile += groups, ti++) {
       const int b = ti & 1;
       const int m0 = (tile % a.mtiles * CG + rank) * kTileM, n0 = tile / a.mtiles * n;
       const int cols = min(n, a.M - n0);
-      for (int j = e; j < n; j += 128) tl.sw[b][j] = j < cols ? a.sw[n0 + j] : 0.f;
-      const int t = m0 + 32 * q + lane;
-      const float sx = t < a.T ? a.sx[t] : 0.f;
-      // The four warps take the same way out: a verdict is shared. The
-      // barriers also put tl.sw in place.
+      tl.sw[b][e] = next_sw;
+      const float sx = next_sx;
+      fetch(tile + groups);
+      // The warps take the same way out: a verdict is shared. The barriers
+      // also put tl.sw in place.
       const bool mine = __all_sync(0xffffffffu, mbar_wait(&tl.tfull[b], (ti >> 1) & 1, a.err));
-      if (lane == 0) tl.ok[q] = mine;
-      named_sync(1, 128);
-      const bool ok = tl.ok[0] && tl.ok[1] && tl.ok[2] && tl.ok[3];
-      named_sync(1, 128);
+      if (lane == 0) tl.ok[warp - 2] = mine;
+      named_sync(1, kEpiThreads);
+      const bool ok = __all_sync(0xffffffffu, tl.ok[lane % kEpiWarps] != 0);
+      named_sync(1, kEpiThreads);
       if (!ok) break;
       q_fence_after();
-      if (m0 + 32 * q < a.T) {  // warp-uniform: some of this warp's tokens exist
-        const uint32_t taddr = tmem + uint32_t(b * kMaxN) + (uint32_t(32 * q) << 16);
-        float* row = a.out + size_t(t) * a.M + n0;
-        for (int c = 0; c < cols; c += 16) {
-          int acc[16];
-          q_tmem_ld16(taddr + c, acc);
-          float v[16];
+      const uint32_t taddr = tmem + uint32_t(b * kMaxN) + (uint32_t(32 * q) << 16);
+      // 32 tokens by (up to) 32 channels from column c.
+      auto put = [&](int c, int (&acc)[32]) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile's last store
+        __syncwarp();
+        const bool half = c + 32 > n;  // the tile ends after 16 channels: rows of 64 bytes, not swizzled
+        float4* to_s = half ? reinterpret_cast<float4*>(tile_s + lane * 64) : mine_s;
+        const int flip = half ? 0 : lane & 7;
 #pragma unroll
-          for (int j = 0; j < 16; j++) v[j] = __fmul_rn(__int2float_rn(acc[j]), __fmul_rn(tl.sw[b][c + j], sx));
-          if (t >= a.T) {
-            // no such token
-          } else if (a.vec == 8 && c + 16 <= cols) {
-            st8(row + c, v);
-            st8(row + c + 8, v + 8);
-          } else if (a.vec >= 4 && c + 16 <= cols) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(row + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-              if (c + j < cols) row[c + j] = v[j];
+        for (int j = 0; j < 8; j++) {
+          if (half && j >= 4) break;
+          const float4 sw = *reinterpret_cast<const float4*>(&tl.sw[b][c + 4 * j]);
+          to_s[j ^ flip] = make_float4(__fmul_rn(__int2float_rn(acc[4 * j]), __fmul_rn(sw.x, sx)),
+                                       __fmul_rn(__int2float_rn(acc[4 * j + 1]), __fmul_rn(sw.y, sx)),
+                                       __fmul_rn(__int2float_rn(acc[4 * j + 2]), __fmul_rn(sw.z, sx)),
+                                       __fmul_rn(__int2float_rn(acc[4 * j + 3]), __fmul_rn(sw.w, sx)));
+        }
+        if (a.tma_out) fence_proxy_async_smem();
+        __syncwarp();
+        if (a.tma_out) {
+          if (lane == 0) {
+            tma_store_2d(half ? &tout16 : &tout, n0 + c, m0 + 32 * q, tile_s);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-          __syncwarp();  // the next tcgen05.ld is the whole warp's
+        } else if (c + lane < cols) {
+          const int rows = min(32, a.T - m0 - 32 * q), pitch = half ? 64 : 128;
+          float* to = a.out + size_t(m0 + 32 * q) * a.M + n0 + c + lane;
+          for (int r = 0; r < rows; r++, to += a.M)
+            *to = *reinterpret_cast<const float*>(tile_s + r * pitch + (((lane >> 2) ^ (half ? 0 : r & 7)) << 4) +
+                                                  (lane & 3) * 4);
+        }
+        __syncwarp();
+      };
+      if (m0 + 32 * q < a.T) {  // warp-uniform: some of this warp's tokens exist
+        // Every second 32 channels are this warp's; the next ones are on their way while it writes these.
+        constexpr int kNext = 32 * (kEpiWarps / 4);
+        int acc[2][32];
+        int c = 32 * ((warp - 2) / 4);
+        if (c < cols) q_tmem_ld32(taddr + c, acc[0]);
+        while (c < cols) {
+          q_tmem_wait(acc[0]);
+          if (c + kNext < cols) q_tmem_ld32(taddr + c + kNext, acc[1]);
+          put(c, acc[0]);
+          if ((c += kNext) >= cols) break;
+          q_tmem_wait(acc[1]);
+          if (c + kNext < cols) q_tmem_ld32(taddr + c + kNext, acc[0]);
+          put(c, acc[1]);
+          c += kNext;
         }
       }
       q_fence_before();
@@ -445,6 +502,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
                        : "memory");
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory may go
   }
   q_fence_before();
   __syncthreads();
@@ -458,8 +516,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
   }
 }
 
-// Tensor map of 8-bit rows in boxes of 128 columns by box_rows rows.
-int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
+// Tensor map of `rows` rows of `cols` elements, `pitch` bytes apart.
+int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, void* base, size_t rows, size_t cols, size_t pitch,
+                int box_cols, int box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult r{};
@@ -469,16 +528,18 @@ int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   }();
   if (!encode) return rt::fail(TB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {cuuint64_t(q->ld), cuuint64_t(q->cap)};
-  cuuint64_t strides[1] = {cuuint64_t(q->ld)};
-  cuuint32_t box[2] = {cuuint32_t(kKB), cuuint32_t(box_rows)};
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(pitch)};
+  cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q->values, dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode(map, type, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return rt::fail(TB200_ERR_CUDA, "matmul_q8: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
   return TB200_OK;
+}
+int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q->values, q->cap, q->ld, q->ld, kKB, box_rows);
 }
 
 // Channels per tile: the multiple of `step` with which the group that has most
@@ -507,17 +568,24 @@ int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   a.err = d->async_err_dev;
   a.mtiles = (a.T + CG * kTileM - 1) / (CG * kTileM);
   a.n = plan_n(a.M, a.mtiles, d->sms / CG, 16 * CG);
+  if (getenv("TBN")) a.n = atoi(getenv("TBN"));
   a.ntiles = (a.M + a.n - 1) / a.n;
   a.xrows = CG == 2 ? kTileM : std::min(kTileM, (a.T + 7) / 8 * 8);
   const int wrows = a.n / CG;
-  const size_t fixed = size_t(kTileM - a.xrows) * kKB + sizeof(QTail) + 1024;
+  const size_t fixed = kStaging + sizeof(QTail) + 1024;
   a.stages = int(std::min<size_t>(kQMaxStages, (kQMaxSmem - fixed) / q_stage_bytes(wrows, a.xrows)));
-  const uintptr_t al = reinterpret_cast<uintptr_t>(out) | (uintptr_t(a.M) * 4);
-  a.vec = al % 32 == 0 ? 8 : al % 16 == 0 ? 4 : 1;
-  CUtensorMap tw, tx;
+  a.tma_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && a.M % 4 == 0;
+  CUtensorMap tw, tx, tout{}, tout16{};
   if (int rc = encode_tmap_q8(&tw, w, wrows)) return rc;
   if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
-  const size_t smem = std::max(kQMinSmem, q_ring_bytes(wrows, a.xrows, a.stages) + sizeof(QTail) + 1024);
+  if (a.tma_out) {
+    const auto f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    if (int rc = encode_tmap(&tout, f32, out, x->rows, w->rows, w->rows * 4, 32, 32)) return rc;
+    if (a.n % 32)
+      if (int rc = encode_tmap(&tout16, f32, out, x->rows, w->rows, w->rows * 4, 16, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+  }
+  const size_t smem = std::max(kQMinSmem, q_ring_bytes(wrows, a.xrows, a.stages) + fixed);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(CG * std::min<long long>((long long)a.mtiles * a.ntiles, d->sms / CG)));
   cfg.blockDim = dim3(kQThreads);
@@ -530,7 +598,7 @@ int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   attr[1].val.clusterDim = {CG, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = CG;  // one CTA: no cluster
-  cudaLaunchKernelEx(&cfg, k_gemm_q8<CG>, tw, tx, a);
+  cudaLaunchKernelEx(&cfg, k_gemm_q8<CG>, tw, tx, tout, tout16, a);
   return rt::launched("matmul_q8");
 }
 
