@@ -220,11 +220,15 @@ def test_resized_rows(b200):
 
 PRODUCTS = [
     # tokens, channels, columns
-    (1, 1, 1), (1, 5, 16), (1, 4096, 1024), (1, 33, 1001), (1, 1000, 10240), (2, 128, 128), (3, 257, 96), (4, 9, 2560),
+    (3, 17000, 2600), (4, 40001, 1100), (1, 1, 1), (1, 5, 16), (1, 4096, 1024), (1, 33, 1001), (1, 1000, 10240), (2, 128, 128), (3, 257, 96), (4, 9, 2560),
     (5, 300, 130), (7, 131, 777), (8, 1024, 512), (9, 640, 2560), (15, 40, 3000), (16, 128, 64), (17, 129, 1001),
     (31, 1000, 31), (33, 77, 4100), (48, 4096, 1024), (63, 2560, 96), (64, 640, 2560), (65, 130, 200), (100, 1, 100),
     (128, 1024, 1024), (129, 513, 640), (200, 2560, 257), (256, 256, 9728), (300, 1200, 1100), (511, 1023, 511),
     (513, 3001, 160), (1025, 260, 384), (2050, 130, 48),
+    # a long K over few channels, cut over the CTAs of a cluster
+    (64, 2560, 9728), (20, 1001, 5000), (130, 300, 4000), (8, 100, 20000), (5, 16, 1025), (128, 2000, 2048),
+    # pairs of CTAs: a second CTA with no tokens, with some, odd channels
+    (1100, 515, 2100), (1025, 260, 2048), (1290, 64, 2500), (1999, 1000, 2176),
 ]
 
 

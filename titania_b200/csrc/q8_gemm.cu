@@ -43,10 +43,11 @@ namespace tb {
 namespace {
 constexpr size_t kMaxCols = 131071;  // 128 * 128 * 131071 < 2^31
 
-// A warp per R channels and up to kVecTokens tokens: R rows' loads are on their
-// way at once.
-constexpr int kVecTokens = 4;
-template <int T, int R>
+// S warps per R channels, for T tokens. Rows are read in the order they lie in
+// memory by many warps with two 16-byte pieces each on their way: six or eight
+// of them, or more channels a warp, are slower (one token, 151936 x 1024: 24.3 us,
+// 27.4 with predicated batches; 2560 x 9728: 7.8 and 9.7).
+template <int T, int R, int S>
 __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, const int8_t* __restrict__ w,
                                                    const float* __restrict__ sw, int channels,
                                                    const int8_t* __restrict__ x, const float* __restrict__ sx, int ldw,
@@ -54,8 +55,8 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c0 = (blockIdx.x * 8 + warp) * R;
-  if (c0 >= channels) return;
+  const int c0 = (blockIdx.x * 8 + warp) / S * R;
+  if (S == 1 && c0 >= channels) return;
   int acc[R][T];
   const int4* wr[R];
 #pragma unroll
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
   }
   const int n = ldw / 16;
 #pragma unroll 2
-  for (int i = lane; i < n; i += 32) {
+  for (int i = lane + 32 * (warp % S); i < n; i += 32 * S) {
     int4 a[R];
 #pragma unroll
     for (int r = 0; r < R; r++) a[r] = __ldcs(wr[r] + i);
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
       }
     }
   }
-  int mine = 0;
+  int mine = 0;  // lane t R + r: channel r, token t
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
@@ -90,6 +91,14 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
       const int s = __reduce_add_sync(0xffffffffu, acc[r][t]);
       if (lane == t * R + r) mine = s;
     }
+  if constexpr (S > 1) {
+    __shared__ int parts[8][R * T];
+    if (lane < R * T) parts[warp][lane] = mine;
+    __syncthreads();
+    if (warp % S) return;
+    if (lane < R * T)
+      for (int s = 1; s < S; s++) mine += parts[warp + s][lane];
+  }
   const int c = c0 + lane % R, t = lane / R;
   if (t < T && c < channels)
     out[size_t(t) * channels + c] = __fmul_rn(__int2float_rn(mine), __fmul_rn(sw[c], sx[t]));
@@ -98,11 +107,19 @@ __global__ void __launch_bounds__(256) k_matvec_q8(float* __restrict__ out, cons
 template <int T>
 void matvec_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   const int channels = int(w->rows);
-  auto go = [&](auto kernel, int r) {
-    launch_pdl(kernel, dim3(unsigned((channels + 8 * r - 1) / (8 * r))), dim3(256), 0, d->stream, out, w->values,
-               w->scales, channels, x->values, x->scales, int(w->ld), int(x->ld));
+  // One channel a warp for one token, two for more, which halves the reads of x.
+  constexpr int R = T == 1 ? 1 : 2;
+  auto go = [&](auto kernel, int s) {
+    const int each = 8 / s * R;  // channels of a block
+    launch_pdl(kernel, dim3(unsigned((channels + each - 1) / each)), dim3(256), 0, d->stream, out, w->values, w->scales,
+               channels, x->values, x->scales, int(w->ld), int(x->ld));
   };
-  go(k_matvec_q8<T, T == 1 ? 1 : 2>, T == 1 ? 1 : 2);
+  // Two warps share the rows where there would be fewer than 28 warps an SM (us: one token, 2560 x 9728
+  // 7.7 with one and 5.9 with two; 6000 x 4096 5.6 and 5.9; four tokens, 4096 x 1024 2.5 and 2.1).
+  if (channels / R < 28 * d->sms)
+    go(k_matvec_q8<T, R, 2>, 2);
+  else
+    go(k_matvec_q8<T, R, 1>, 1);
 }
 
 // ---- tensor cores ------------------------------------------------------------
@@ -125,7 +142,10 @@ struct QGemmArgs {
   int n;             // channels per tile
   int xrows;         // token rows per tile that are loaded (a multiple of 8, at most 128)
   int stages, mtiles, ntiles;
+  int splits;        // SPLIT: CTAs that share a tile's sums
   int tma_out;       // output rows begin on 16-byte boundaries: a TMA store can write them
+  unsigned ring;     // bytes of the ring
+  unsigned recv;     // SPLIT: bytes of the other CTAs' sums
   int* err;
 };
 
@@ -136,7 +156,7 @@ constexpr size_t kStaging = size_t(kEpiWarps) * kStageTile;
 // Shared memory after the ring and the staging: barriers full[s], empty[s], tfull[2], tempty[2],
 // mdone, then the address of the tensor memory and the epilogue's scales.
 struct QTail {
-  uint64_t full[kQMaxStages], empty[kQMaxStages], tfull[2], tempty[2], mdone;
+  uint64_t full[kQMaxStages], empty[kQMaxStages], tfull[2], tempty[2], mdone, summed;
   uint32_t tmem;
   int ok[kEpiWarps];
   alignas(16) float sw[2][kMaxN];
@@ -244,7 +264,7 @@ __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, int* e
     }
   }
 }
-__device__ __forceinline__ void pair_sync() {
+__device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -273,13 +293,32 @@ __device__ __forceinline__ void tma_store_2d(const void* map, int x, int y, cons
                : "memory");
 }
 
+// Copies from this CTA's shared memory to the same cluster's CTA `rank`,
+// completing on a barrier there.
+__device__ __forceinline__ void bulk_to_cta(const void* dst, const void* src, uint32_t bytes, const uint64_t* bar,
+                                            uint32_t rank) {
+  uint32_t d, b;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(dst)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(d),
+               "r"(smem_u32(src)), "r"(bytes), "r"(b)
+               : "memory");
+}
+
 // CG CTAs work on a tile of 128 CG tokens by n channels. A pair (CG = 2) sits
 // on neighbouring SMs: each CTA loads its 128 tokens and half of the channels,
 // the first one's MMA warp issues MMAs of 256 tokens over both CTAs' shared
 // memory, and each CTA finds its tokens' sums in its own tensor memory. Per
 // output that takes two thirds of one CTA's bytes from L2, which is what
 // bounds many tokens.
-template <int CG>
+//
+// SPLIT: the sums of a tile are cut over the CTAs of a cluster (a.splits of
+// them), one tile a cluster. An MMA takes at least 64 cycles, the time to read
+// its 128 token rows, so narrow tiles over all of a long K waste it. The CTAs
+// take turns in the tile's units of 32 tokens by 32 channels: each copies its
+// sums of a unit to the unit's CTA (4 KB by a bulk copy; reading them there
+// word by word took 13000 cycles), which adds them up and writes them.
+template <int CG, bool SPLIT>
 __global__ void __launch_bounds__(kQThreads, 1)
     k_gemm_q8(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
               const __grid_constant__ CUtensorMap tout, const __grid_constant__ CUtensorMap tout16, QGemmArgs a) {
@@ -288,16 +327,25 @@ __global__ void __launch_bounds__(kQThreads, 1)
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles: 1024-byte alignment
   const int stages = a.stages, n = a.n, wrows = n / CG;
   const uint32_t stage_bytes = uint32_t(q_stage_bytes(wrows, a.xrows));
-  unsigned char* staging = sm + q_ring_bytes(wrows, a.xrows, stages);
-  QTail& tl = *reinterpret_cast<QTail*>(staging + kStaging);
+  unsigned char* staging = sm + a.ring;
+  unsigned char* recv = staging + kStaging;  // SPLIT: the other CTAs' sums, [this CTA's units][CTA]
+  QTail& tl = *reinterpret_cast<QTail*>(recv + a.recv);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  static_assert(CG == 1 || !SPLIT, "a split tile is one CTA wide");
   const int rank = CG == 2 ? int(pair_rank()) : 0;
-  const int group = int(blockIdx.x) / CG, groups = int(gridDim.x) / CG;
-  const int nkb = (a.K + kKB - 1) / kKB;
+  const int per = SPLIT ? a.splits : CG, part = SPLIT ? int(pair_rank()) : 0;
+  const int group = int(blockIdx.x) / per, groups = int(gridDim.x) / per;
+  // The 128-column steps of K of this CTA: kb0 .. kb0 + nkb.
+  const int all_kb = (a.K + kKB - 1) / kKB;
+  const int kb0 = SPLIT ? int((long long)all_kb * part / a.splits) : 0;
+  const int nkb = SPLIT ? int((long long)all_kb * (part + 1) / a.splits) - kb0 : all_kb;
   const int tiles = a.mtiles * a.ntiles;
+  // SPLIT: units of the tile, quarter by quarter of its tokens within 32 channels.
+  const int quarters = SPLIT ? (min(kTileM, a.T - group % a.mtiles * kTileM) + 31) / 32 : 0;
+  const int units = SPLIT ? (min(n, a.M - group / a.mtiles * n) + 31) / 32 * quarters : 0;
   // Each group begins its sums at another place of K: the order is free, and
   // CTAs that share token rows do not all ask the same L2 slices for them at once.
-  const int k0 = int((long long)group * nkb / groups);
+  const int k0 = SPLIT ? 0 : int((long long)group * nkb / groups);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
@@ -309,6 +357,11 @@ __global__ void __launch_bounds__(kQThreads, 1)
       mbar_init(&tl.tempty[b], kEpiWarps * CG);  // one arrival per epilogue warp
     }
     mbar_init(&tl.mdone, 1);
+    if constexpr (SPLIT) {
+      mbar_init(&tl.summed, 1);
+      const int mine = (units - part + a.splits - 1) / a.splits;
+      mbar_arrive_expect_tx(&tl.summed, uint32_t(mine * (a.splits - 1) * kStageTile));
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -330,11 +383,50 @@ __global__ void __launch_bounds__(kQThreads, 1)
   }
   q_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) pair_sync();  // both CTAs' barriers and tensor memory are there
+  if constexpr (CG == 2 || SPLIT) cluster_sync();  // every CTA's barriers and tensor memory are there
   q_fence_after();
   const uint32_t tmem = tl.tmem;
   pdl_launch_dependents();
   pdl_wait();
+
+        // Epilogue warps: scales and writes the sums of 32 tokens (quarter q of the
+  // tile at m0) by up to 32 channels from column c of the tile at n0, a lane a
+  // token, through this warp's staging tile, where 16-byte piece j of a row
+  // lies at j ^ (row & 7). b: which of tl.sw.
+  unsigned char* tile_s = staging + (warp - 2) * kStageTile;
+  float4* mine_s = reinterpret_cast<float4*>(tile_s + lane * 128);
+        auto put = [&](int b, int m0, int n0, int q, int c, float sx, int (&acc)[32]) {
+      const int cols = min(n, a.M - n0);
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile's last store
+          __syncwarp();
+          const bool half = c + 32 > n;  // the tile ends after 16 channels: rows of 64 bytes, not swizzled
+          float4* to_s = half ? reinterpret_cast<float4*>(tile_s + lane * 64) : mine_s;
+          const int flip = half ? 0 : lane & 7;
+  #pragma unroll
+          for (int j = 0; j < 8; j++) {
+            if (half && j >= 4) break;
+            const float4 sw = *reinterpret_cast<const float4*>(&tl.sw[b][c + 4 * j]);
+            to_s[j ^ flip] = make_float4(__fmul_rn(__int2float_rn(acc[4 * j]), __fmul_rn(sw.x, sx)),
+                                         __fmul_rn(__int2float_rn(acc[4 * j + 1]), __fmul_rn(sw.y, sx)),
+                                         __fmul_rn(__int2float_rn(acc[4 * j + 2]), __fmul_rn(sw.z, sx)),
+                                         __fmul_rn(__int2float_rn(acc[4 * j + 3]), __fmul_rn(sw.w, sx)));
+          }
+          if (a.tma_out) fence_proxy_async_smem();
+          __syncwarp();
+          if (a.tma_out) {
+            if (lane == 0) {
+              tma_store_2d(half ? &tout16 : &tout, n0 + c, m0 + 32 * q, tile_s);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else if (c + lane < cols) {
+            const int rows = min(32, a.T - m0 - 32 * q), pitch = half ? 64 : 128;
+            float* to = a.out + size_t(m0 + 32 * q) * a.M + n0 + c + lane;
+            for (int r = 0; r < rows; r++, to += a.M)
+              *to = *reinterpret_cast<const float*>(tile_s + r * pitch + (((lane >> 2) ^ (half ? 0 : r & 7)) << 4) +
+                                                    (lane & 3) * 4);
+          }
+          __syncwarp();
+        };
 
   // The producer's and the MMA warp's lanes stay together and one of them is
   // elected at each instruction: what they issue takes uniform registers, and
@@ -352,7 +444,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
           ok = false;
           break;
         }
-        const int at = (k + k0 < nkb ? k + k0 : k + k0 - nkb) * kKB;
+        const int at = (kb0 + (k + k0 < nkb ? k + k0 : k + k0 - nkb)) * kKB;
         unsigned char *dw = sm + size_t(s) * stage_bytes, *dx = dw + size_t(wrows) * kKB;
         if (elect_one()) {
           // The first CTA's barrier counts both CTAs' bytes, of which the second's may come before it
@@ -413,9 +505,6 @@ __global__ void __launch_bounds__(kQThreads, 1)
     const int q = warp & 3;  // the 32 accumulator lanes this warp can read
     const int e = int(threadIdx.x) - 64;
     int ti = 0;
-    // This lane's row of the warp's staging tile: 16-byte piece j lies at j ^ (row & 7).
-    unsigned char* tile_s = staging + (warp - 2) * kStageTile;
-    float4* mine_s = reinterpret_cast<float4*>(tile_s + lane * 128);
     // The scales of a tile are fetched while the one before is written.
     static_assert(kEpiThreads == kMaxN, "a channel's scale for each thread");
     float next_sw = 0.f, next_sx = 0.f;
@@ -443,52 +532,38 @@ __global__ void __launch_bounds__(kQThreads, 1)
       if (!ok) break;
       q_fence_after();
       const uint32_t taddr = tmem + uint32_t(b * kMaxN) + (uint32_t(32 * q) << 16);
-      // 32 tokens by (up to) 32 channels from column c.
-      auto put = [&](int c, int (&acc)[32]) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile's last store
-        __syncwarp();
-        const bool half = c + 32 > n;  // the tile ends after 16 channels: rows of 64 bytes, not swizzled
-        float4* to_s = half ? reinterpret_cast<float4*>(tile_s + lane * 64) : mine_s;
-        const int flip = half ? 0 : lane & 7;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          if (half && j >= 4) break;
-          const float4 sw = *reinterpret_cast<const float4*>(&tl.sw[b][c + 4 * j]);
-          to_s[j ^ flip] = make_float4(__fmul_rn(__int2float_rn(acc[4 * j]), __fmul_rn(sw.x, sx)),
-                                       __fmul_rn(__int2float_rn(acc[4 * j + 1]), __fmul_rn(sw.y, sx)),
-                                       __fmul_rn(__int2float_rn(acc[4 * j + 2]), __fmul_rn(sw.z, sx)),
-                                       __fmul_rn(__int2float_rn(acc[4 * j + 3]), __fmul_rn(sw.w, sx)));
-        }
-        if (a.tma_out) fence_proxy_async_smem();
-        __syncwarp();
-        if (a.tma_out) {
-          if (lane == 0) {
-            tma_store_2d(half ? &tout16 : &tout, n0 + c, m0 + 32 * q, tile_s);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else if (c + lane < cols) {
-          const int rows = min(32, a.T - m0 - 32 * q), pitch = half ? 64 : 128;
-          float* to = a.out + size_t(m0 + 32 * q) * a.M + n0 + c + lane;
-          for (int r = 0; r < rows; r++, to += a.M)
-            *to = *reinterpret_cast<const float*>(tile_s + r * pitch + (((lane >> 2) ^ (half ? 0 : r & 7)) << 4) +
-                                                  (lane & 3) * 4);
-        }
-        __syncwarp();
-      };
       if (m0 + 32 * q < a.T) {  // warp-uniform: some of this warp's tokens exist
         // Every second 32 channels are this warp's; the next ones are on their way while it writes these.
         constexpr int kNext = 32 * (kEpiWarps / 4);
         int acc[2][32];
         int c = 32 * ((warp - 2) / 4);
+        auto give = [&](int (&v)[32]) {
+          if constexpr (SPLIT) {
+            // Where the ring was: every load has landed and every MMA has read it.
+            const int u = c / 32 * quarters + q, owner = u % a.splits;
+            unsigned char* sums = sm + size_t(u) * kStageTile;
+            int4* to = reinterpret_cast<int4*>(sums + lane * 128);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              to[j ^ (lane & 7)] = make_int4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (owner != part && lane == 0)
+              bulk_to_cta(recv + size_t(u / a.splits * a.splits + part) * kStageTile, sums, kStageTile, &tl.summed,
+                          uint32_t(owner));
+          } else {
+            put(b, m0, n0, q, c, sx, v);
+          }
+        };
         if (c < cols) q_tmem_ld32(taddr + c, acc[0]);
         while (c < cols) {
           q_tmem_wait(acc[0]);
           if (c + kNext < cols) q_tmem_ld32(taddr + c + kNext, acc[1]);
-          put(c, acc[0]);
+          give(acc[0]);
           if ((c += kNext) >= cols) break;
           q_tmem_wait(acc[1]);
           if (c + kNext < cols) q_tmem_ld32(taddr + c + kNext, acc[0]);
-          put(c, acc[1]);
+          give(acc[1]);
           c += kNext;
         }
       }
@@ -502,11 +577,33 @@ __global__ void __launch_bounds__(kQThreads, 1)
                        : "memory");
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory may go
   }
+  if constexpr (SPLIT) {
+    __syncthreads();  // this CTA's own sums are in its shared memory
+    if (warp >= 2 && __all_sync(0xffffffffu, mbar_wait(&tl.summed, 0, a.err))) {
+      const int m0 = group % a.mtiles * kTileM, n0 = group / a.mtiles * n;
+      for (int i = warp - 2; part + i * a.splits < units; i += kEpiWarps) {
+        const int u = part + i * a.splits, q = u % quarters, c = u / quarters * 32, t = m0 + 32 * q + lane;
+        int acc[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) acc[j] = 0;
+        for (int r = 0; r < a.splits; r++) {
+          const unsigned char* from =
+              r == part ? sm + size_t(u) * kStageTile : recv + size_t(i * a.splits + r) * kStageTile;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const int4 v = *reinterpret_cast<const int4*>(from + lane * 128 + ((j ^ (lane & 7)) << 4));
+            acc[4 * j] += v.x, acc[4 * j + 1] += v.y, acc[4 * j + 2] += v.z, acc[4 * j + 3] += v.w;
+          }
+        }
+        put(0, m0, n0, q, c, t < a.T ? a.sx[t] : 0.f, acc);
+      }
+    }
+  }
+  if (warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory may go
   q_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) pair_sync();  // no MMA reads the other CTA's memory, no arrival is on its way there
+  if constexpr (CG == 2 || SPLIT) cluster_sync();  // nothing reads or signals the other CTAs' memory any more
   if (warp == 1) {
     q_fence_after();
     if constexpr (CG == 1)
@@ -542,21 +639,98 @@ int encode_tmap_q8(CUtensorMap* map, const tb200_q8* q, int box_rows) {
   return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q->values, q->cap, q->ld, q->ld, kKB, box_rows);
 }
 
-// Channels per tile: the multiple of `step` with which the group that has most
-// to do has least, a tile's fixed cost (filling the ring, the last tile's
-// epilogue) counted as 24 channels.
-int plan_n(int M, int mtiles, int groups, int step) {
-  int best = 0;
+struct QPlan {
+  int n, splits;
+};
+// One CTA a tile: the channels (a multiple of 16) with which the CTA that has
+// most to do has least, a tile's fixed cost (filling the ring, the last tile's
+// epilogue) counted as 24 channels. Where the tiles leave SMs idle, the sums
+// may be cut over two or four CTAs instead: in cycles, a step of K takes four MMAs
+// of n / 2, at least 64, and a cluster and its adding up about 5000 (64 x 2560 x
+// 9728: 14.2 us uncut, 9.5 cut over four; 64 x 1024 x 2048: 4.9 and 5.7). Clusters
+// of eight CTAs of this size do not all run at once: 18 and 10.7 us.
+constexpr size_t kQFixed = kStaging + sizeof(QTail) + 1024;
+// Bytes of sums that a CTA of a split tile receives, by the quarters of its tokens.
+size_t q_recv_bytes(int n, int splits, int quarters) {
+  const int units = (n + 31) / 32 * quarters;
+  return size_t((units + splits - 1) / splits) * splits * kStageTile;
+}
+int q_stages(int wrows, int xrows, size_t recv) {
+  return int(std::min<size_t>(kQMaxStages, (kQMaxSmem - kQFixed - recv) / q_stage_bytes(wrows, xrows)));
+}
+QPlan plan_one(int M, int nkb, int T, int sms) {
+  const int mtiles = (T + kTileM - 1) / kTileM, xrows = std::min(kTileM, (T + 7) / 8 * 8), quarters = (xrows + 31) / 32;
+  QPlan best{0, 1};
   long long least = 0;
-  for (int n = step; n <= kMaxN; n += step) {
+  for (int n = 16; n <= kMaxN; n += 16) {
     const long long tiles = (long long)mtiles * ((M + n - 1) / n);
-    const long long cost = (tiles + groups - 1) / groups * (n + 24);
-    if (!best || cost <= least) best = n, least = cost;
+    const long long cost = (tiles + sms - 1) / sms * (n + 24);
+    if (!best.n || cost <= least) best.n = n, least = cost;
+  }
+  const long long tiles = (long long)mtiles * ((M + best.n - 1) / best.n);
+  long long cycles = (tiles + sms - 1) / sms * nkb * 4 * std::max(64, best.n / 2);
+  for (int splits = 2; splits <= 4 && splits <= nkb; splits *= 2)
+    for (int n = 32; n <= 160; n += 16) {
+      if (q_stages(n, xrows, q_recv_bytes(n, splits, quarters)) < 3) continue;
+      // A cluster lies within one of the groups of SMs that a GPU is made of, which it need not divide.
+      if ((long long)mtiles * ((M + n - 1) / n) * splits > sms - sms * splits / 64) continue;
+      const long long c = (long long)((nkb + splits - 1) / splits) * 4 * std::max(64, n / 2) + 5000;
+      if (c < cycles) best = {n, splits}, cycles = c;
+    }
+  return best;
+}
+// Pairs of CTAs (n a multiple of 32): bound by loads, so a step counts as its rows.
+QPlan plan_pair(int M, int mtiles, int pairs) {
+  QPlan best{0, 1};
+  long long least = 0;
+  for (int n = 32; n <= kMaxN; n += 32) {
+    const long long tiles = (long long)mtiles * ((M + n - 1) / n);
+    const long long cost = (tiles + pairs - 1) / pairs * (n / 2 + kTileM);
+    if (!best.n || cost <= least) best.n = n, least = cost;
   }
   return best;
 }
 
-template <int CG>
+template <int CG, bool SPLIT>
+int launch_gemm_q8(tb200_device* d, QGemmArgs a, QPlan p, const tb200_q8* w, const tb200_q8* x) {
+  a.mtiles = (a.T + CG * kTileM - 1) / (CG * kTileM);
+  a.n = p.n;
+  a.splits = p.splits;
+  a.ntiles = (a.M + a.n - 1) / a.n;
+  a.xrows = CG == 2 ? kTileM : std::min(kTileM, (a.T + 7) / 8 * 8);
+  const int wrows = a.n / CG;
+  a.recv = SPLIT ? unsigned(q_recv_bytes(a.n, a.splits, (a.xrows + 31) / 32)) : 0;
+  a.stages = q_stages(wrows, a.xrows, a.recv);
+  CUtensorMap tw, tx, tout{}, tout16{};
+  if (int rc = encode_tmap_q8(&tw, w, wrows)) return rc;
+  if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
+  if (a.tma_out) {
+    const auto f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    if (int rc = encode_tmap(&tout, f32, a.out, x->rows, w->rows, w->rows * 4, 32, 32)) return rc;
+    if (a.n % 32)
+      if (int rc = encode_tmap(&tout16, f32, a.out, x->rows, w->rows, w->rows * 4, 16, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+  }
+  // The ring also holds a split tile's sums.
+  const size_t sums = SPLIT ? size_t((a.n + 31) / 32) * ((a.xrows + 31) / 32) * kStageTile : 0;
+  a.ring = unsigned(std::max(q_ring_bytes(wrows, a.xrows, a.stages), sums));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = SPLIT ? dim3(unsigned(a.mtiles * a.ntiles * p.splits))
+                      : dim3(unsigned(CG * std::min<long long>((long long)a.mtiles * a.ntiles, d->sms / CG)));
+  cfg.blockDim = dim3(kQThreads);
+  cfg.dynamicSmemBytes = std::max(kQMinSmem, a.ring + a.recv + kQFixed);
+  cfg.stream = d->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {unsigned(SPLIT ? p.splits : CG), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 || SPLIT ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, k_gemm_q8<CG, SPLIT>, tw, tx, tout, tout16, a);
+  return rt::launched("matmul_q8");
+}
+
 int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   QGemmArgs a{};
   a.sw = w->scales;
@@ -566,48 +740,22 @@ int gemm_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x) {
   a.M = int(w->rows);
   a.K = int(w->cols);
   a.err = d->async_err_dev;
-  a.mtiles = (a.T + CG * kTileM - 1) / (CG * kTileM);
-  a.n = plan_n(a.M, a.mtiles, d->sms / CG, 16 * CG);
-  if (getenv("TBN")) a.n = atoi(getenv("TBN"));
-  a.ntiles = (a.M + a.n - 1) / a.n;
-  a.xrows = CG == 2 ? kTileM : std::min(kTileM, (a.T + 7) / 8 * 8);
-  const int wrows = a.n / CG;
-  const size_t fixed = kStaging + sizeof(QTail) + 1024;
-  a.stages = int(std::min<size_t>(kQMaxStages, (kQMaxSmem - fixed) / q_stage_bytes(wrows, a.xrows)));
   a.tma_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && a.M % 4 == 0;
-  CUtensorMap tw, tx, tout{}, tout16{};
-  if (int rc = encode_tmap_q8(&tw, w, wrows)) return rc;
-  if (int rc = encode_tmap_q8(&tx, x, a.xrows)) return rc;
-  if (a.tma_out) {
-    const auto f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    if (int rc = encode_tmap(&tout, f32, out, x->rows, w->rows, w->rows * 4, 32, 32)) return rc;
-    if (a.n % 32)
-      if (int rc = encode_tmap(&tout16, f32, out, x->rows, w->rows, w->rows * 4, 16, 32, CU_TENSOR_MAP_SWIZZLE_NONE))
-        return rc;
-  }
-  const size_t smem = std::max(kQMinSmem, q_ring_bytes(wrows, a.xrows, a.stages) + fixed);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(CG * std::min<long long>((long long)a.mtiles * a.ntiles, d->sms / CG)));
-  cfg.blockDim = dim3(kQThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = d->stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {CG, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = CG;  // one CTA: no cluster
-  cudaLaunchKernelEx(&cfg, k_gemm_q8<CG>, tw, tx, tout, tout16, a);
-  return rt::launched("matmul_q8");
+  // Pairs take fewer bytes from L2 but wait for one another: 1999 x 9728 x 2560 takes 43.8 us with
+  // pairs and 47.8 without, 512 x 4096 x 1024 6.9 and 5.7.
+  if (a.T >= 1024 && a.K >= 2048)
+    return launch_gemm_q8<2, false>(d, a, plan_pair(a.M, (a.T + 2 * kTileM - 1) / (2 * kTileM), d->sms / 2), w, x);
+  const QPlan p = plan_one(a.M, (a.K + kKB - 1) / kKB, a.T, d->sms);
+  return p.splits > 1 ? launch_gemm_q8<1, true>(d, a, p, w, x) : launch_gemm_q8<1, false>(d, a, p, w, x);
 }
 
 }  // namespace
 
 cudaError_t init_q8_kernels() {
-  cudaError_t e = cudaFuncSetAttribute(k_gemm_q8<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(k_gemm_q8<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kQMaxSmem));
+  const auto most = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(k_gemm_q8<1, false>, most, int(kQMaxSmem));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_gemm_q8<1, true>, most, int(kQMaxSmem));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_gemm_q8<2, false>, most, int(kQMaxSmem));
   return e;
 }
 
@@ -624,12 +772,14 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   ARG_CHECK(out->len == x->rows * w->rows, "matmul_q8: output holds " + std::to_string(out->len) + ", expected " +
                                                std::to_string(x->rows * w->rows));
   if (!x->rows || !w->rows) return TB200_OK;
+  // Three or four tokens over many weights keep the CUDA cores busy for longer than the weights take to
+  // arrive (four tokens, us: 151936 x 1024 33.6 there and 28.1 on the tensor cores, 2560 x 9728 8.4 and 9.4).
+  if (x->rows > 4 || (x->rows > 2 && w->rows * w->cols >= size_t(40) << 20)) return tb::gemm_q8(d, out->ptr, w, x);
   switch (x->rows) {
     case 1: tb::matvec_q8<1>(d, out->ptr, w, x); break;
     case 2: tb::matvec_q8<2>(d, out->ptr, w, x); break;
     case 3: tb::matvec_q8<3>(d, out->ptr, w, x); break;
-    case 4: tb::matvec_q8<4>(d, out->ptr, w, x); break;
-    default: return x->rows > 128 && !getenv("TB1") ? tb::gemm_q8<2>(d, out->ptr, w, x) : tb::gemm_q8<1>(d, out->ptr, w, x);
+    default: tb::matvec_q8<4>(d, out->ptr, w, x);
   }
   return rt::launched("matmul_q8");
 }
