@@ -124,8 +124,9 @@ def test_one_token_has_almost_everything(b200):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [1, 9])
 @pytest.mark.parametrize("vocab", [40, 1000, 70001])
-def test_rows_that_are_not_ordinary(b200, vocab):
+def test_rows_that_are_not_ordinary(b200, vocab, top):
     """Excluded tokens (-inf), rows of nothing else, NaN of either sign,
     infinities, zeros of either sign, the type's lowest and largest values."""
     rng = np.random.default_rng(vocab)
@@ -142,17 +143,17 @@ def test_rows_that_are_not_ordinary(b200, vocab):
     x[9], x[9, 3] = np.finfo(F32).min, 2.0
     x[10], x[10, 4], x[10, 5] = np.finfo(F32).max, 0.0, np.finfo(F32).min
     x[11, 1:] = -np.inf
-    s = tb.LogProbs(b200, 12, vocab, 9)
+    s = tb.LogProbs(b200, 12, vocab, top)
     for tokens in ([1] * 12, [17] * 12, [0] * 12, list(range(12))):
         got = s.score(buf(b200, x), tokens)
-        lp, ent, ids, tops = reference(x, tokens, 9)
+        lp, ent, ids, tops = reference(x, tokens, top)
         assert got[2].tolist() == ids.tolist()
         for g, e in ((got[0], lp), (got[1], ent), (got[3], tops)):
             assert np.array_equal(np.isnan(g), np.isnan(e))
             assert np.array_equal(np.isneginf(g), np.isneginf(e))
             ok = np.isfinite(e)
             # f32's lowest against ordinary numbers: relative to the difference
-            assert np.all(np.abs(g - e)[ok] <= CHAIN * EPS * (2 + np.abs(e[ok])))
+            assert np.all(np.abs(g[ok] - e[ok]) <= CHAIN * EPS * (2 + np.abs(e[ok])))
 
 
 @pytest.mark.gpu
@@ -160,8 +161,24 @@ def test_orders_of_rising_and_falling_logits(b200):
     """All of the alternatives next to one another, at either end."""
     vocab = 151936
     x = np.stack([np.arange(vocab), -np.arange(vocab), np.arange(vocab) // 500]).astype(F32) * F32(1e-3)
-    s = tb.LogProbs(b200, 3, vocab, 64)
-    compare(s.score(buf(b200, x), [5, 5, 5]), x, [5, 5, 5], 64)
+    for top in (64, 20, 1):
+        s = tb.LogProbs(b200, 3, vocab, top)
+        compare(s.score(buf(b200, x), [5, 5, 5]), x, [5, 5, 5], top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [0, 1, 2, 30])
+def test_many_rows_of_every_alignment(b200, top):
+    """More rows than CTAs, rows that start anywhere within 16 bytes, ties
+    between the parts of a row; twice the same bits."""
+    rng = np.random.default_rng(top)
+    x = np.round(rng.standard_normal((1301, 2053)) * 2).astype(F32)
+    tokens = rng.integers(0, 2053, 1301)
+    s, b = tb.LogProbs(b200, 1301, 2053, top), buf(b200, x)
+    got = s.score(b, tokens)
+    compare(got, x, tokens, top)
+    for a, c in zip(got, s.score(b, tokens)):
+        assert np.array_equal(a.view(np.int32), c.view(np.int32))
 
 
 @pytest.mark.gpu

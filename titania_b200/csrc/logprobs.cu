@@ -27,8 +27,8 @@
 // element of another block), so only those are read again; the same goes for
 // the granules of four logits among them. That is a few microseconds a row of
 // waiting more than of work: with few rows the CTA that finishes a row does it,
-// with many it is a kernel of its own with a CTA for every row (1111 rows, one
-// alternative: 131 us in one kernel, of which 20 are theirs).
+// with many it is a kernel of its own with a CTA for every row. One alternative
+// is the maximum itself, whose place the warps keep.
 #include <algorithm>
 #include <climits>
 #include <string>
@@ -43,8 +43,9 @@ struct tb200_scorer {
   uint32_t* top_ids = nullptr;
   uint32_t* tokens = nullptr;   // [rows] ids given in host memory
   float4* part = nullptr;       // sums of the pieces
-  int* block_max = nullptr;     // [rows][a row's blocks], when there are alternatives
-  float2* peak = nullptr;       // [rows] maximum and log Z, when there are alternatives
+  unsigned long long* part_best = nullptr;  // their largest logits, when there is one alternative
+  int* block_max = nullptr;     // [rows][a row's blocks], when there are several
+  float2* peak = nullptr;       // [rows] maximum and log Z, likewise
   unsigned* ticket = nullptr;   // [rows], zero between launches
   int ctas = 0;                 // that the GPU runs at once
 };
@@ -263,9 +264,10 @@ struct ScoreArgs {
   float *logprob, *entropy, *top_logprobs;
   uint32_t* top_ids;
   float4* part;     // piece of row r by CTA c: [r + c]
-  int* block_max;   // [rows][steps * kStep]
+  unsigned long long* part_best;  // its largest logit, likewise
+  int* block_max;   // [rows][steps * kStep], or null
   unsigned* ticket;
-  float2* peak;     // [rows] maximum and log Z for k_alternatives, or null
+  float2* peak;     // [rows] maximum and log Z for k_alternatives
   int vocab, top;
   int steps;        // of a row, whatever its alignment
   long long total;  // steps of all rows
@@ -278,6 +280,7 @@ struct ScoreShared {
   int first[kScoreWarps];
   int counts[2][kScoreWarps];
   uint2 range[kScoreWarps];
+  unsigned long long best[kScoreWarps];
   unsigned long long cand[kCand];
   int blocks[kPicked];
 };
@@ -467,6 +470,12 @@ __device__ __forceinline__ Soft soft_cta(const Soft& p, int warp, int lane, Scor
   return soft_lanes(sh.soft[lane % kScoreWarps], kScoreWarps, lane);
 }
 
+// What a call does about the alternatives: nothing, or what k_alternatives needs
+// (the table and a.peak, where a.block_max is given); the one most likely token, which
+// is the place of the maximum and needs no table; several, by the CTA that
+// finishes a row.
+enum ScoreTop { kTopApart, kTopOne, kTopMany };
+template <int TOP>
 __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
   __shared__ ScoreShared sh;
   pdl_launch_dependents();
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     const int s0 = int(g - (long long)row * a.steps), s1 = int(min((long long)a.steps, s0 + (g1 - g)));
     g += s1 - s0;
     const Row r(a.logits, row, a.vocab);
-    int* block_max = a.top ? a.block_max + row * size_t(a.steps) * kStep : nullptr;
+    int* block_max = TOP != kTopOne && a.block_max ? a.block_max + row * size_t(a.steps) * kStep : nullptr;
     // The token's logit, for whoever finishes the row: on its way while the others are read.
     float given = nan;
     if (threadIdx.x == 0) {
@@ -491,6 +500,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     bool whole = false;
     float x[kStep][4], met = 0.f;
     int bm[kStep], top = INT_MIN;
+    unsigned long long best = 0;  // kTopOne: the largest logit, if this warp met it
     auto load = [&] {
       const int b = st * kStep;
       whole = r.inside(b) && r.inside(b + kStep - 1);
@@ -505,6 +515,16 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
       });
       if (block_max && lane == 0) reinterpret_cast<int4*>(block_max)[st] = make_int4(bm[0], bm[1], bm[2], bm[3]);
     };
+    // kTopOne: the step's largest is larger than all before it; its first place.
+    auto keep = [&] {
+      unsigned at = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = kStep * 4 - 1; i >= 0; i--) {
+        const int e = r.element(st * kStep + i / 4, lane, i % 4);
+        if (order(x[i / 4][i % 4]) == top && e >= 0 && e < a.vocab) at = unsigned(e);
+      }
+      best = order_key(top, __reduce_min_sync(0xffffffffu, at));
+    };
     if (st < s1) load();
     if (lane == 0) sh.first[warp] = top;
     __syncthreads();
@@ -513,11 +533,16 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     common = __shfl_sync(0xffffffffu, common, __ffs(holders) - 1);
     Running run(max(common, kNegInf));
     if (st < s1) {
-      step_add(run, x, lane, warp == __ffs(holders) - 1);
+      const bool holder = warp == __ffs(holders) - 1;
+      if (TOP == kTopOne && holder) keep();
+      step_add(run, x, lane, holder);
       for (st += kScoreWarps; st < s1; st += kScoreWarps) {
         load();
         const bool higher = top > run.order;
-        if (higher) run.raise(top, lane);
+        if (higher) {
+          run.raise(top, lane);
+          if (TOP == kTopOne) keep();
+        }
         step_add(run, x, lane, higher);
       }
     }
@@ -525,12 +550,15 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     Soft s = run.settled();
     s.s = warp_sum(s.s);
     s.t = warp_sum(s.t);
+    if (TOP == kTopOne && lane == 0) sh.best[warp] = best;
     s = soft_cta(s, warp, lane, sh);
+    if (TOP == kTopOne) best = warp_umax64(sh.best[lane % kScoreWarps]);
     // Pieces of this row: those of the CTAs whose runs meet it.
     const long long c0 = (long long)row * a.steps / a.run, c1 = ((long long)(row + 1) * a.steps - 1) / a.run;
     if (c1 > c0) {
       if (threadIdx.x == 0) {
         a.part[row + blockIdx.x] = make_float4(s.m, s.s, s.t, s.own);
+        if (TOP == kTopOne) a.part_best[row + blockIdx.x] = best;
         unsigned before;  // releases this CTA's writes, acquires those of the CTAs before it
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.ticket + row) : "memory");
         sh.last = before == unsigned(c1 - c0);
@@ -544,8 +572,14 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
       for (long long c = c0 + threadIdx.x; c <= c1; c += kScoreThreads) {
         const float4 q = __ldcg(a.part + row + c);
         p = soft_join(p, Soft{q.x, q.y, q.z, q.w});
+        if (TOP == kTopOne) best = max(best, __ldcg(a.part_best + row + c));
+      }
+      if (TOP == kTopOne) {
+        best = warp_umax64(best);
+        if (lane == 0) sh.best[warp] = best;
       }
       s = soft_cta(soft_lanes(p, 32, lane), warp, lane, sh);
+      if (TOP == kTopOne) best = warp_umax64(sh.best[lane % kScoreWarps]);
       if (threadIdx.x == 0) a.ticket[row] = 0;
     }
     const bool bad = !(s.m < INFINITY) || s.m == -INFINITY || isnan(s.s);
@@ -553,12 +587,14 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     if (threadIdx.x == 0) {
       a.entropy[row] = logz + kLn2 * s.t / (1.0f + s.s);
       a.logprob[row] = (given - s.m) - logz;
+      if (TOP == kTopOne) {
+        a.top_ids[row] = argmax_index(best);
+        a.top_logprobs[row] = (unorder(int(uint32_t(best >> 32) ^ 0x80000000u)) - s.m) - logz;
+      } else if (TOP == kTopApart && a.block_max) {
+        a.peak[row] = make_float2(s.m, logz);
+      }
     }
-    if (a.peak) {
-      if (threadIdx.x == 0) a.peak[row] = make_float2(s.m, logz);
-    } else if (a.top) {
-      alternatives(a, r, row, s.m, logz, sh);
-    }
+    if constexpr (TOP == kTopMany) alternatives(a, r, row, s.m, logz, sh);
     __syncthreads();  // shared memory is free for the next piece
   }
 }
@@ -594,7 +630,7 @@ int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, t
   s->top = int(top);
   const size_t blocks = size_t(tb::score_steps(vocab)) * tb::kStep;
   int per_sm = 0;
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, tb::k_score, tb::kScoreThreads, 0);
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, tb::k_score<tb::kTopMany>, tb::kScoreThreads, 0);
   s->ctas = std::max(1, per_sm) * dev->sms;
   const size_t parts = rows + size_t(s->ctas);
   if (e == cudaSuccess) e = cudaMalloc(&s->logprob, rows * 4);
@@ -605,8 +641,9 @@ int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, t
   if (e == cudaSuccess) e = cudaMalloc(&s->part, parts * sizeof(float4));
   if (e == cudaSuccess) e = cudaMalloc(&s->ticket, rows * 4);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->ticket, 0, rows * 4, dev->stream);
-  if (e == cudaSuccess && top) e = cudaMalloc(&s->block_max, rows * blocks * 4);
-  if (e == cudaSuccess && top) e = cudaMalloc(&s->peak, rows * sizeof(float2));
+  if (e == cudaSuccess && top == 1) e = cudaMalloc(&s->part_best, parts * 8);
+  if (e == cudaSuccess && top > 1) e = cudaMalloc(&s->block_max, rows * blocks * 4);
+  if (e == cudaSuccess && top > 1) e = cudaMalloc(&s->peak, rows * sizeof(float2));
   if (e == cudaSuccess) e = cudaMemsetAsync(s->logprob, 0, rows * 4, dev->stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->entropy, 0, rows * 4, dev->stream);
   if (e == cudaSuccess && top) e = cudaMemsetAsync(s->top_ids, 0, rows * top * 4, dev->stream);
@@ -630,6 +667,7 @@ int tb200_scorer_free(tb200_scorer* s) {
   cudaFree(s->top_ids);
   cudaFree(s->top_logprobs);
   cudaFree(s->part);
+  cudaFree(s->part_best);
   cudaFree(s->block_max);
   cudaFree(s->peak);
   cudaFree(s->ticket);
@@ -677,10 +715,18 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.total = (long long)n * a.steps;
   // Equal runs for the CTAs that run at once, of a step for every warp at least where rows are that long.
   a.run = std::max<long long>((a.total + s->ctas - 1) / s->ctas, std::min(a.steps, tb::kScoreWarps));
-  // More rows than half the CTAs: some would find alternatives while others wait for the rest of their run.
-  a.peak = 2 * n > size_t(s->ctas) ? s->peak : nullptr;
-  tb::launch_pdl(tb::k_score, dim3(unsigned((a.total + a.run - 1) / a.run)), dim3(tb::kScoreThreads), 0, st, a);
-  if (a.peak) tb::launch_pdl(tb::k_alternatives, dim3(unsigned(n)), dim3(tb::kScoreThreads), 0, st, a);
+  a.part_best = s->part_best;
+  a.peak = s->peak;
+  const dim3 grid(unsigned((a.total + a.run - 1) / a.run)), block(tb::kScoreThreads);
+  if (s->top == 1) {
+    tb::launch_pdl(tb::k_score<tb::kTopOne>, grid, block, 0, st, a);
+  } else if (s->top && 2 * n <= size_t(s->ctas)) {
+    tb::launch_pdl(tb::k_score<tb::kTopMany>, grid, block, 0, st, a);
+  } else {
+    // More rows than half the CTAs: some would find alternatives while others wait for the rest of their run.
+    tb::launch_pdl(tb::k_score<tb::kTopApart>, grid, block, 0, st, a);
+    if (s->top) tb::launch_pdl(tb::k_alternatives, dim3(unsigned(n)), block, 0, st, a);
+  }
   return rt::launched("score");
 }
 
