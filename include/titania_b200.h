@@ -198,7 +198,7 @@ TB200_API int tb200_silu_mul(tb200_device* dev, tb200_buffer* gate, const tb200_
  * whose scale f32 does not hold, has scale NaN and zeros: every product with
  * it is NaN. */
 
-/* A handle of `rows` (0 or more) rows of `cols` (1 .. 2^31 - 1) values, all zero. */
+/* A handle of `rows` (0 .. 2^30) rows of `cols` (1 .. 2^30) values, all zero. */
 TB200_API int tb200_q8_new(tb200_device* dev, size_t rows, size_t cols, tb200_q8** out);
 TB200_API int tb200_q8_free(tb200_device* dev, tb200_q8* q);
 /* Changes the number of rows, up to the number it was made with; what the
@@ -478,7 +478,7 @@ TB200_API int tb200_sampler_state(tb200_sampler* sampler, uint64_t* out);
 /* ---- log probabilities (no counterpart in the reference) ------------------- */
 
 /* What a scorer holds: room for `rows` rows of results over logits of
- * `vocab` values (1 .. 2^31 - 1), and the `top` (0 .. 64, at most vocab)
+ * `vocab` values (1 .. 2^30), and the `top` (0 .. 64, at most vocab)
  * most likely alternatives of each. */
 TB200_API int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, tb200_scorer** out);
 TB200_API int tb200_scorer_free(tb200_scorer* s);

@@ -251,7 +251,8 @@ def test_tokens_on_the_device_and_captured(b200):
 
 @pytest.mark.gpu
 def test_refusals(b200):
-    for rows, vocab, top in ((0, 10, 1), (1, 0, 0), (1, 10, 11), (1, 1000, 65)):
+    for rows, vocab, top in ((0, 10, 1), (1, 0, 0), (1, 10, 11), (1, 1000, 65), (1, 2 ** 30 + 1, 0),
+                             (2 ** 24 + 1, 10, 0)):
         with pytest.raises(tb.DeviceError, match="bad|top"):
             tb.LogProbs(b200, rows, vocab, top)
     s, b = tb.LogProbs(b200, 2, 100, 3), b200.alloc(200)

@@ -311,6 +311,10 @@ def test_refusals(b200):
     q, x, w = b200.q8(4, 64), b200.alloc(4 * 64), b200.upload(tb.Tensor([64], np.zeros(64, np.uint16)))
     with pytest.raises(tb.DeviceError, match="columns"):
         b200.q8(1, 0)
+    with pytest.raises(tb.DeviceError, match="columns"):
+        b200.q8(0, 2 ** 30 + 1)
+    with pytest.raises(tb.DeviceError, match="rows"):
+        b200.q8(2 ** 30 + 1, 1)
     with pytest.raises(tb.DeviceError, match="expected 256"):
         b200.quantize(q, b200.alloc(255))
     with pytest.raises(tb.DeviceError, match="expected 256"):

@@ -11,24 +11,27 @@
 // Both terms of the entropy are positive and log1p keeps S's relative error,
 // so neither loses digits when one token has almost all of the probability.
 //
-// One launch, one pass over the logits, bound by reading them. The rows' steps
-// of 512 logits, one after another, are dealt out to the CTAs in equal runs
-// (whatever the number of rows, no SM waits for another's last row); a CTA's
-// part of a row is a piece. A warp takes a step at a time, as four blocks of
-// 128: their largest, a redux each, are both the running maximum that the sums
-// refer to and the blocks' entries in a table of 1/128 of the logits' size. The
-// warps of a CTA begin a piece with the largest of their first steps as common
-// maximum, so that few steps raise it: that takes a warp-uniform branch as
-// dear as the step itself. Per logit there are five instructions for the sums
-// and one for the maximum; at ten it was bound by them (1111 x 151936: 142 us,
-// against 105 us for the bytes). The CTA that finishes a row's last piece joins the pieces'
-// sums, in their order. The alternatives: the k largest logits lie in the k blocks
-// with the largest maxima (each of those has an element at least as large as any
-// element of another block), so only those are read again; the same goes for
-// the granules of four logits among them. That is a few microseconds a row of
-// waiting more than of work: with few rows the CTA that finishes a row does it,
-// with many it is a kernel of its own with a CTA for every row. One alternative
-// is the maximum itself, whose place the warps keep.
+// One pass over the logits, bound by reading them (1111 x 151936: 110 us, of
+// which the bytes take 105). The rows' steps of 512 logits, one after another, are
+// dealt out to the CTAs that run at once in equal runs (whatever the number of
+// rows, no SM waits for another's last one); a CTA's part of a row is a piece. A
+// warp takes a step at a time, as four blocks of 128: their largest, a redux each,
+// are both the running maximum that the sums refer to and the blocks' entries in
+// a table of 1/128 of the logits' size. The warps of a CTA begin a piece with the
+// largest of their first steps as common maximum, so that few steps raise it:
+// that is a warp-uniform branch as dear as a step. Per logit there are five
+// instructions for the sums and one for the maximum; at ten the kernel was bound
+// by them (142 us). The CTA that finishes a row's last piece joins the pieces'
+// sums, in their order.
+//
+// The alternatives: the k largest logits lie in the k blocks with the largest
+// maxima (each of those has an element at least as large as any element of
+// another block), so only those are read again. That is a few microseconds a row,
+// of waiting more than of work: with few rows the CTA that finishes a row does it
+// (64 rows, five alternatives: 16 us, 11.5 with none), with many it is a kernel of
+// its own with a CTA for every row (1111 rows: 125 us; in one kernel 131). One warp
+// alone takes 20 us for it. One alternative is the maximum itself, whose place
+// the warps keep (117 us).
 #include <algorithm>
 #include <climits>
 #include <string>
@@ -620,7 +623,7 @@ extern "C" {
 int tb200_scorer_new(tb200_device* dev, size_t rows, size_t vocab, size_t top, tb200_scorer** out) {
   ARG_CHECK(dev && out, "null argument");
   ARG_CHECK(rows >= 1 && rows <= (size_t(1) << 24), "bad number of rows");
-  ARG_CHECK(vocab >= 1 && vocab < (size_t(1) << 31), "bad vocabulary");
+  ARG_CHECK(vocab >= 1 && vocab <= (size_t(1) << 30), "bad vocabulary");
   ARG_CHECK(top <= size_t(tb::kScoreMaxTop) && top <= vocab, "top must be at most 64 and the vocabulary");
   if (int rc = rt::use(dev)) return rc;
   auto* s = new tb200_scorer;

@@ -412,7 +412,7 @@ RowArgs row_args(const tb200_q8* out) {
 
 namespace {
 
-constexpr size_t kMaxDim = (size_t(1) << 31) - 1;
+constexpr size_t kMaxDim = size_t(1) << 30;  // 32-bit indices along a row, and of rows in tiles
 
 void q8_release(tb200_q8* q) {
   cudaFree(q->values);
@@ -427,7 +427,7 @@ extern "C" {
 int tb200_q8_new(tb200_device* d, size_t rows, size_t cols, tb200_q8** out) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(out, "null output handle");
-  ARG_CHECK(cols > 0 && cols <= kMaxDim - 15, "q8: bad number of columns");
+  ARG_CHECK(cols > 0 && cols <= kMaxDim, "q8: bad number of columns");
   ARG_CHECK(rows <= kMaxDim, "q8: too many rows");
   auto* q = new tb200_q8;
   q->rows = q->cap = rows;
