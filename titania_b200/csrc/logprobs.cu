@@ -379,12 +379,25 @@ __device__ __noinline__ void granule_candidates(const Row& r, int k, int& turn, 
   __syncthreads();
 }
 
-// The `top` largest of a row with maximum m, ranked: by the whole CTA.
+__device__ __forceinline__ const int* row_table(const ScoreArgs& a, size_t row) {
+  return a.block_max + row * size_t(a.steps) * kStep;
+}
+// A thread's entries of the row's table, where all of them fit the CTA's registers.
+__device__ __forceinline__ void table_entries(const ScoreArgs& a, const Row& r, size_t row, int (&entry)[kOwn]) {
+#pragma unroll
+  for (int i = 0; i < kOwn; i++) {
+    const int b = int(threadIdx.x) + i * kScoreThreads;
+    entry[i] = r.blocks <= kOwn * kScoreThreads && b < r.blocks ? __ldcg(row_table(a, row) + b) : 0;
+  }
+}
+
+// The `top` largest of a row with maximum m, ranked: by the whole CTA, whose
+// table_entries() are there.
 __device__ __forceinline__ void alternatives(const ScoreArgs& a, const Row& r, size_t row, float m, float logz,
-                                             ScoreShared& sh) {
+                                             const int (&entry)[kOwn], ScoreShared& sh) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k = a.top;
-  const int* block_max = a.block_max + row * size_t(a.steps) * kStep;
+  const int* block_max = row_table(a, row);
   int turn = 0;
   if (threadIdx.x == 0) sh.n_blocks = sh.n_cand = 0;
   // The blocks with the largest maxima: k of them, or more where that ends the search sooner.
@@ -396,7 +409,7 @@ __device__ __forceinline__ void alternatives(const ScoreArgs& a, const Row& r, s
 #pragma unroll
     for (int i = 0; i < kOwn; i++) {
       const int b = int(threadIdx.x) + i * kScoreThreads;
-      own[i] = b < r.blocks ? block_key(b) : 0ull;
+      own[i] = b < r.blocks ? order_key(entry[i], uint32_t(b)) : 0ull;
     }
     bound = own_bound(kb, own, r.blocks, turn, sh);
     __syncthreads();
@@ -557,6 +570,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     s = soft_cta(s, warp, lane, sh);
     if (TOP == kTopOne) best = warp_umax64(sh.best[lane % kScoreWarps]);
     // Pieces of this row: those of the CTAs whose runs meet it.
+    int entry[kOwn];
     const long long c0 = (long long)row * a.steps / a.run, c1 = ((long long)(row + 1) * a.steps - 1) / a.run;
     if (c1 > c0) {
       if (threadIdx.x == 0) {
@@ -571,6 +585,8 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
         __syncthreads();  // sh.last is read before the next piece writes it
         continue;
       }
+      // On their way while the sums are joined.
+      if (TOP == kTopMany) table_entries(a, r, row, entry);
       Soft p{-INFINITY, 0.f, 0.f, 0.f};
       for (long long c = c0 + threadIdx.x; c <= c1; c += kScoreThreads) {
         const float4 q = __ldcg(a.part + row + c);
@@ -584,6 +600,8 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
       s = soft_cta(soft_lanes(p, 32, lane), warp, lane, sh);
       if (TOP == kTopOne) best = warp_umax64(sh.best[lane % kScoreWarps]);
       if (threadIdx.x == 0) a.ticket[row] = 0;
+    } else if (TOP == kTopMany) {
+      table_entries(a, r, row, entry);
     }
     const bool bad = !(s.m < INFINITY) || s.m == -INFINITY || isnan(s.s);
     const float logz = bad ? nan : log1pf(s.s);
@@ -597,7 +615,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
         a.peak[row] = make_float2(s.m, logz);
       }
     }
-    if constexpr (TOP == kTopMany) alternatives(a, r, row, s.m, logz, sh);
+    if constexpr (TOP == kTopMany) alternatives(a, r, row, s.m, logz, entry, sh);
     __syncthreads();  // shared memory is free for the next piece
   }
 }
@@ -608,8 +626,11 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_alternatives(ScoreArgs a) 
   pdl_launch_dependents();
   pdl_wait();
   const size_t row = blockIdx.x;
+  const Row r(a.logits, row, a.vocab);
+  int entry[kOwn];
+  table_entries(a, r, row, entry);
   const float2 p = a.peak[row];
-  alternatives(a, Row(a.logits, row, a.vocab), row, p.x, p.y, sh);
+  alternatives(a, r, row, p.x, p.y, entry, sh);
 }
 
 // Steps of a row, whatever its alignment.

@@ -14,17 +14,24 @@
 // channels so that the tiles come out even over the SMs.
 //   warp 0     producer: per 128 columns of K, a box of up to 128 token rows
 //              and one of N channel rows (128-byte swizzle) into a ring;
-//   warp 1     one lane issues the MMAs (K = 32 each), commits each stage back
-//              to the producer and each tile to the epilogue;
-//   warps 2-9  epilogue, two for each 32 lanes of the accumulator: tcgen05.ld, scales, then 32 x 32 outputs at a time
-//              through shared memory (128-byte swizzle) into a TMA store; two
-//              accumulators let it run behind the next tile's MMAs. With 32-byte
-//              stores from each lane's own row it took 450 to 790 cycles for 16
-//              columns, longer than the MMAs of a tile up to K = 2560.
+//   warp 1     issues the MMAs (K = 32 each), commits each stage back to the
+//              producer and each tile to the epilogue;
+//   warps 2-9  epilogue, two for each 32 lanes of the accumulator: tcgen05.ld,
+//              scales, then 32 x 32 outputs at a time through shared memory
+//              (128-byte swizzle) into a TMA store; two accumulators let it run
+//              behind the next tile's MMAs. With 32-byte stores from each lane's
+//              own row it took 450 to 790 cycles for 16 columns, longer than
+//              the MMAs of a tile up to K = 2560.
 // Persistent CTAs walk the tiles, token tiles innermost, so that a channel
-// tile comes from memory once. Only the token rows that exist are loaded: the
-// MMA reads whatever shared memory holds in the place of the others, and the
-// accumulator rows that this makes are never read.
+// tile comes from memory once; many tokens go to pairs of CTAs, long sums over
+// few channels to clusters that share a tile's K (below). Only the token rows
+// that exist are loaded: the MMA reads whatever shared memory holds in the place
+// of the others, and the accumulator rows that this makes are never read.
+//
+// Measured (us; memory or bf16-rate floor): 64 x 19456 x 2560 11.6 (8.5), of which
+// filling the ring and the last tile's way out take 3; 1999 x 9728 x 2560 43.8 (58.8;
+// 2.3 P operations/s, bound by the 50 to 70 bytes a clock that a SM's loads reach),
+// 51 back to back under the power cap; 64 x 2560 x 9728 9.5 (4.1).
 //
 // Every mbarrier wait is bounded (kWaitCycles); on expiry the kernel leaves
 // TB200_ERR_TIMEOUT in the device's async error word, lets what it issued
@@ -153,8 +160,8 @@ struct QGemmArgs {
 constexpr int kStageTile = 32 * 128;
 constexpr size_t kStaging = size_t(kEpiWarps) * kStageTile;
 
-// Shared memory after the ring and the staging: barriers full[s], empty[s], tfull[2], tempty[2],
-// mdone, then the address of the tensor memory and the epilogue's scales.
+// Shared memory after the ring, the staging and what a split tile receives:
+// barriers, then the address of the tensor memory and the epilogue's scales.
 struct QTail {
   uint64_t full[kQMaxStages], empty[kQMaxStages], tfull[2], tempty[2], mdone, summed;
   uint32_t tmem;
@@ -263,6 +270,10 @@ __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, int* e
       return false;
     }
   }
+}
+// The same verdict for the whole warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -440,7 +451,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
     for (int tile = group; tile < tiles && ok; tile += groups) {
       const int m0 = (tile % a.mtiles * CG + rank) * kTileM, n0 = tile / a.mtiles * n + rank * wrows;
       for (int k = 0; k < nkb; k++, i++) {
-        if (!mbar_wait(&tl.empty[s], phase, a.err)) {
+        if (!warp_wait(&tl.empty[s], phase, a.err)) {
           ok = false;
           break;
         }
@@ -477,11 +488,13 @@ __global__ void __launch_bounds__(kQThreads, 1)
         const int b = ti & 1;
         // The epilogue has drained this accumulator's previous tile.
         const uint32_t drained = ((ti >> 1) - 1) & 1;
-        if (!(CG == 1 ? mbar_wait(&tl.tempty[b], drained, a.err) : pair_wait(&tl.tempty[b], drained, a.err))) break;
+        if (!(CG == 1 ? warp_wait(&tl.tempty[b], drained, a.err)
+                      : __all_sync(0xffffffffu, pair_wait(&tl.tempty[b], drained, a.err))))
+          break;
         q_fence_after();
         const uint32_t acc = tmem + uint32_t(b * kMaxN);
         for (int k = 0; k < nkb; k++) {
-          if (!mbar_wait(&tl.full[s], phase, a.err)) {
+          if (!warp_wait(&tl.full[s], phase, a.err)) {
             ok = false;
             break;
           }
@@ -524,7 +537,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
       fetch(tile + groups);
       // The warps take the same way out: a verdict is shared. The barriers
       // also put tl.sw in place.
-      const bool mine = __all_sync(0xffffffffu, mbar_wait(&tl.tfull[b], (ti >> 1) & 1, a.err));
+      const bool mine = warp_wait(&tl.tfull[b], (ti >> 1) & 1, a.err);
       if (lane == 0) tl.ok[warp - 2] = mine;
       named_sync(1, kEpiThreads);
       const bool ok = __all_sync(0xffffffffu, tl.ok[lane % kEpiWarps] != 0);
@@ -580,7 +593,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
   }
   if constexpr (SPLIT) {
     __syncthreads();  // this CTA's own sums are in its shared memory
-    if (warp >= 2 && __all_sync(0xffffffffu, mbar_wait(&tl.summed, 0, a.err))) {
+    if (warp >= 2 && warp_wait(&tl.summed, 0, a.err)) {
       const int m0 = group % a.mtiles * kTileM, n0 = group / a.mtiles * n;
       for (int i = warp - 2; part + i * a.splits < units; i += kEpiWarps) {
         const int u = part + i * a.splits, q = u % quarters, c = u / quarters * 32, t = m0 + 32 * q + lane;
