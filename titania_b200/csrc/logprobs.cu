@@ -68,6 +68,7 @@ constexpr int kCand = 4 * kPicked;            // elements of as many granules
 constexpr int kOwn = 8;                       // table entries a thread keeps in registers
 constexpr int kGranules = 13;                 // granules of the picked blocks that it keeps
 static_assert(kPicked * 32 <= kGranules * kScoreThreads, "they fit");
+constexpr int kOneByOne = 6;                  // alternatives of a short row that are found in turn
 constexpr int kNegInf = int(0xFF800000u ^ 0x7FFFFFFFu);  // order(-inf)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -633,6 +634,141 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_alternatives(ScoreArgs a) 
   alternatives(a, r, row, p.x, p.y, entry, sh);
 }
 
+// Short rows, of at most S steps: a warp each, the whole row in its registers; no
+// pieces, no barriers. A few alternatives are the largest remaining logit, time
+// after time; more are those above a bound, ranked (1400 x 500: 8 us with five, 10
+// with twenty, which took 19 one by one; by CTAs 36).
+template <int S>
+__global__ void __launch_bounds__(kScoreThreads) k_score_rows(ScoreArgs a, int rows) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * kScoreWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const Row r(a.logits, size_t(row), a.vocab);
+  const float nan = __int_as_float(0x7FC00000);
+  const uint32_t tok = a.tokens[row];
+  const float given = tok < uint32_t(a.vocab) ? __ldg(r.base + r.shift + tok) : nan;
+  float x[S][kStep][4], met = 0.f;
+  int top[S], common = INT_MIN;
+#pragma unroll
+  for (int s = 0; s < S; s++)
+#pragma unroll
+    for (int u = 0; u < kStep; u++) {
+      const int b = s * kStep + u;
+      const float4 v = r.inside(b) ? r.load(b, lane) : r.load_end(b, lane, -INFINITY);
+      x[s][u][0] = v.x, x[s][u][1] = v.y, x[s][u][2] = v.z, x[s][u][3] = v.w;
+    }
+  auto real = [&](int s, int i) {
+    const int at = r.element(s * kStep + i / 4, lane, i % 4);
+    return at >= 0 && at < a.vocab;
+  };
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    int bm[kStep];
+    const bool whole = r.inside(s * kStep) && r.inside(s * kStep + kStep - 1);
+    top[s] = step_max(x[s], bm, met, whole, [&](int u, int j) { return whole || real(s, 4 * u + j); });
+    common = max(common, top[s]);
+  }
+  // The logits in order; what is not the row's is out from the start.
+  int o[S][kStep * 4];
+  unsigned gone[S];
+  if (a.top) {
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      gone[s] = 0;
+#pragma unroll
+      for (int i = 0; i < kStep * 4; i++) {
+        o[s][i] = order(x[s][i / 4][i % 4]);
+        gone[s] |= unsigned(!real(s, i)) << i;
+      }
+    }
+  }
+  Running run(max(common, kNegInf));
+  bool leave = true;
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    const bool here = leave && top[s] == common;
+    step_add(run, x[s], lane, here);
+    leave = leave && !here;
+  }
+  run.s += met * 0.0f;  // a NaN stays
+  Soft f = run.settled();
+  f.s = warp_sum(f.s);
+  f.t = warp_sum(f.t);
+  const bool bad = !(f.m < INFINITY) || f.m == -INFINITY || isnan(f.s);
+  const float logz = bad ? nan : log1pf(f.s);
+  if (lane == 0) {
+    a.entropy[row] = logz + kLn2 * f.t / (1.0f + f.s);
+    a.logprob[row] = (given - f.m) - logz;
+  }
+  // A lane's largest remaining logit: its order and its first place.
+  bool have = false;
+  int best = 0, place = 0;
+  auto largest = [&] {
+    have = false;
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+      for (int i = 0; i < kStep * 4; i++)
+        if (!((gone[s] >> i) & 1) && (!have || o[s][i] > best)) have = true, best = o[s][i], place = s * kStep * 4 + i;
+  };
+  if (a.top) largest();
+  if (a.top > kOneByOne) {
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int i = 0; i < kStep * 4; i++)
+          f(!((gone[s] >> i) & 1) ? order_key(o[s][i], uint32_t(r.element(s * kStep + i / 4, lane, i % 4))) : 0ull);
+    };
+    // None is above the largest; the lanes' largest are 32 keys at or above their least.
+    const unsigned mine = have ? unsigned(best) ^ 0x80000000u : 0u;
+    const unsigned low = __reduce_min_sync(0xffffffffu, mine), high = __reduce_max_sync(0xffffffffu, mine);
+    const unsigned long long lo = a.top <= 32 ? static_cast<unsigned long long>(low) << 32 : 0ull;
+    const unsigned long long hi = (static_cast<unsigned long long>(high) << 32) | 0xFFFFFFFFull;
+    const unsigned long long bound = max(1ull, key_bound(a.top, slack(a.top), lo, hi, [&](unsigned long long key) {
+      int c = 0;
+      each([&](unsigned long long k) { c += k >= key; });
+      return __reduce_add_sync(0xffffffffu, c);
+    }));
+    __shared__ unsigned long long rooms[kScoreWarps][kPicked];
+    unsigned long long* room = rooms[threadIdx.x >> 5];
+    int n = 0;
+    each([&](unsigned long long k) {
+      const unsigned who = __ballot_sync(0xffffffffu, k >= bound);
+      if (k >= bound) room[n + __popc(who & ((1u << lane) - 1))] = k;
+      n += __popc(who);
+    });
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+      const unsigned long long k = room[i];
+      int rank = 0;
+      for (int j = 0; j < n; j++) rank += room[j] > k;
+      if (rank < a.top) {
+        a.top_ids[row * a.top + rank] = argmax_index(k);
+        a.top_logprobs[row * a.top + rank] = (unorder(int(uint32_t(k >> 32) ^ 0x80000000u)) - f.m) - logz;
+      }
+    }
+    return;
+  }
+  for (int k = 0; k < a.top; k++) {
+    // Of the lanes with the warp's largest, the one whose element comes first.
+    const int m = __reduce_max_sync(0xffffffffu, have ? best : INT_MIN);
+    const int e = r.element(place / 4, lane, place % 4);
+    const int first = __reduce_min_sync(0xffffffffu, have && best == m ? e : INT_MAX);
+    if (have && e == first) {
+      a.top_ids[row * a.top + k] = uint32_t(e);
+      a.top_logprobs[row * a.top + k] = (unorder(m) - f.m) - logz;
+#pragma unroll
+      for (int s = 0; s < S; s++)
+        if (place / (kStep * 4) == s) gone[s] |= 1u << (place % (kStep * 4));
+      largest();
+    }
+    __syncwarp();
+  }
+}
+
 // Steps of a row, whatever its alignment.
 int score_steps(size_t vocab) { return int((vocab + 3 + kStep * kBlock - 1) / (kStep * kBlock)); }
 
@@ -742,7 +878,15 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.part_best = s->part_best;
   a.peak = s->peak;
   const dim3 grid(unsigned((a.total + a.run - 1) / a.run)), block(tb::kScoreThreads);
-  if (s->top == 1) {
+  if (a.steps <= 4) {
+    const dim3 warps(unsigned((n + tb::kScoreWarps - 1) / tb::kScoreWarps));
+    if (a.steps == 1)
+      tb::launch_pdl(tb::k_score_rows<1>, warps, block, 0, st, a, int(n));
+    else if (a.steps == 2)
+      tb::launch_pdl(tb::k_score_rows<2>, warps, block, 0, st, a, int(n));
+    else
+      tb::launch_pdl(tb::k_score_rows<4>, warps, block, 0, st, a, int(n));
+  } else if (s->top == 1) {
     tb::launch_pdl(tb::k_score<tb::kTopOne>, grid, block, 0, st, a);
   } else if (s->top && 2 * n <= size_t(s->ctas)) {
     tb::launch_pdl(tb::k_score<tb::kTopMany>, grid, block, 0, st, a);
