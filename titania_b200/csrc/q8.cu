@@ -66,6 +66,7 @@ __device__ __noinline__ int row_int(double v, double r, float s) {
 }
 // The same by a product, except next to the middle of two integers.
 __device__ __forceinline__ int row_int(double v, const RowScale& k) {
+  if (!(k.s > 0.0f)) return 0;
   const double d = v * k.c, q = rint(d);
   return k.sure > 0.f && fabs(fabs(d - q) - 0.5) > 1e-9 ? int(q) : row_int(v, k.r, k.s);
 }
@@ -105,7 +106,7 @@ __device__ __forceinline__ float max_abs(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(b));
   return r;
 }
-// The largest of the lanes' bit patterns (f32 >= 0, or their halves) and of 64-bit ones.
+// The largest of the lanes' 64-bit numbers.
 __device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
   const unsigned hi = __reduce_max_sync(0xffffffffu, unsigned(v >> 32));
   const unsigned lo = __reduce_max_sync(0xffffffffu, unsigned(v >> 32) == hi ? unsigned(v) : 0u);

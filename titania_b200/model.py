@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import json
+import math
 import os
 import sys
 
@@ -630,7 +631,7 @@ class LogProbs:
         if a is None:
             t = np.ascontiguousarray(tokens, dtype=np.uint32).reshape(-1)
             return t.ctypes.data, t.size, t
-        n = int(np.prod(a["shape"]))
+        n = math.prod(a["shape"])
         if a["typestr"] not in ("<i4", "<u4") or (a.get("strides") and n > 1 and (
                 len(a["shape"]) != 1 or a["strides"][0] != 4)):
             raise ValueError("token ids on the device must be contiguous 32-bit integers")
