@@ -6,7 +6,7 @@
 // so its order is free; the two f32 roundings of the scales' product and the
 // final product follow it. Every variant below gives the same bits.
 //
-// k_matvec_q8 (few tokens): a warp per channel, dp4a on CUDA cores.
+// k_matvec_q8 (up to eight tokens over few weights): a warp per channel, dp4a on CUDA cores.
 // k_gemm_q8 (more): tcgen05.mma kind::i8, s8 x s8 into s32 accumulators in
 // tensor memory. Tokens are the rows of the accumulator (M = 128 a CTA),
 // channels its columns (N, a multiple of 16 chosen per call). A lane then
@@ -785,14 +785,20 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   ARG_CHECK(out->len == x->rows * w->rows, "matmul_q8: output holds " + std::to_string(out->len) + ", expected " +
                                                std::to_string(x->rows * w->rows));
   if (!x->rows || !w->rows) return TB200_OK;
-  // Three or four tokens over many weights keep the CUDA cores busy for longer than the weights take to
-  // arrive (four tokens, us: 151936 x 1024 33.6 there and 28.1 on the tensor cores, 2560 x 9728 8.4 and 9.4).
-  if (x->rows > 4 || (x->rows > 2 && w->rows * w->cols >= size_t(40) << 20)) return tb::gemm_q8(d, out->ptr, w, x);
+  // Three to eight tokens over many weights keep the CUDA cores busy for longer than the weights take to arrive
+  // (us there and on the tensor cores: four tokens, 2560 x 9728 8.4 and 9.4, 151936 x 1024 33.6 and 28.1; eight,
+  // 1024 x 2048 3.0 and 4.9, 2560 x 4096 5.9 and 6.9, 9728 x 2560 9.9 and 7.9).
+  if (x->rows > 8 || (x->rows > 2 && x->rows * w->rows * w->cols > size_t(128) << 20))
+    return tb::gemm_q8(d, out->ptr, w, x);
   switch (x->rows) {
     case 1: tb::matvec_q8<1>(d, out->ptr, w, x); break;
     case 2: tb::matvec_q8<2>(d, out->ptr, w, x); break;
     case 3: tb::matvec_q8<3>(d, out->ptr, w, x); break;
-    default: tb::matvec_q8<4>(d, out->ptr, w, x);
+    case 4: tb::matvec_q8<4>(d, out->ptr, w, x); break;
+    case 5: tb::matvec_q8<5>(d, out->ptr, w, x); break;
+    case 6: tb::matvec_q8<6>(d, out->ptr, w, x); break;
+    case 7: tb::matvec_q8<7>(d, out->ptr, w, x); break;
+    default: tb::matvec_q8<8>(d, out->ptr, w, x);
   }
   return rt::launched("matmul_q8");
 }
