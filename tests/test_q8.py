@@ -227,7 +227,7 @@ PRODUCTS = [
     (513, 3001, 160), (1025, 260, 384), (2050, 130, 48),
     # few tokens on both sides of the change to tensor cores
     (5, 9001, 300), (6, 2000, 1001), (6, 9000, 64), (7, 8999, 33), (8, 9002, 272), (5, 27001, 1000), (6, 1500, 15000),
-    (7, 10001, 1930), (8, 17009, 1001),
+    (7, 10001, 1930), (8, 17009, 1001), (8, 1000, 20000), (1, 1001, 3001), (4, 600, 129),
     # a long K over few channels, cut over the CTAs of a cluster
     (64, 2560, 9728), (20, 1001, 5000), (130, 300, 4000), (8, 100, 20000), (5, 16, 1025), (128, 2000, 2048),
     # pairs of CTAs: a second CTA with no tokens, with some, odd channels

@@ -121,9 +121,15 @@ void matvec_q8(tb200_device* d, float* out, const tb200_q8* w, const tb200_q8* x
     launch_pdl(kernel, dim3(unsigned((channels + each - 1) / each)), dim3(256), 0, d->stream, out, w->values, w->scales,
                channels, x->values, x->scales, int(w->ld), int(x->ld));
   };
-  // Two warps share the rows where there would be fewer than 28 warps an SM (us: one token, 2560 x 9728
-  // 7.7 with one and 5.9 with two; 6000 x 4096 5.6 and 5.9; four tokens, 4096 x 1024 2.5 and 2.1).
-  if (channels / R < 28 * d->sms)
+  // Two, four or eight warps share the rows where there would be fewer than 28, 8 or 4 warps an SM (us: one
+  // token, 2560 x 9728 7.7 with one and 5.9 with two, 6000 x 4096 5.6 and 5.9; four tokens, 2560 x 2560 3.6 with
+  // two and 4.4 with four; 1000 x 20000 with two, four and eight, one token 7.9, 5.7 and 4.7, four tokens 14.8,
+  // 8.5 and 5.8; 1024 x 1024, one token, 1.4, 1.4 and 1.8).
+  if (channels / R < 4 * d->sms)
+    go(k_matvec_q8<T, R, 8>, 8);
+  else if (channels / R < 8 * d->sms)
+    go(k_matvec_q8<T, R, 4>, 4);
+  else if (channels / R < 28 * d->sms)
     go(k_matvec_q8<T, R, 2>, 2);
   else
     go(k_matvec_q8<T, R, 1>, 1);
@@ -787,8 +793,10 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   if (!x->rows || !w->rows) return TB200_OK;
   // Three to eight tokens over many weights keep the CUDA cores busy for longer than the weights take to arrive
   // (us there and on the tensor cores: four tokens, 2560 x 9728 8.4 and 9.4, 151936 x 1024 33.6 and 28.1; eight,
-  // 1024 x 2048 3.0 and 4.9, 2560 x 4096 5.9 and 6.9, 9728 x 2560 9.9 and 7.9).
-  if (x->rows > 8 || (x->rows > 2 && x->rows * w->rows * w->cols > size_t(128) << 20))
+  // 1024 x 2048 3.0 and 4.9, 2560 x 4096 5.9 and 6.9, 9728 x 2560 9.9 and 7.9), but few channels make few tiles
+  // (eight tokens, 1000 x 20000 7.2 and 12.3).
+  const bool few = w->rows <= size_t(8) * d->sms;
+  if (x->rows > 8 || (x->rows > 2 && !few && x->rows * w->rows * w->cols > size_t(128) << 20))
     return tb::gemm_q8(d, out->ptr, w, x);
   switch (x->rows) {
     case 1: tb::matvec_q8<1>(d, out->ptr, w, x); break;
