@@ -51,7 +51,7 @@ def compare(got, logits, tokens, top):
         ok = np.isfinite(b)
         assert np.isfinite(a[ok]).all()
         t = np.broadcast_to(t.reshape(t.shape + (1,) * (b.ndim - 1)), b.shape)
-        assert np.all(np.abs(a - b)[ok] <= t[ok]), np.abs(a - b)[ok].max()
+        assert np.all(np.abs(a[ok] - b[ok]) <= t[ok]), np.abs(a[ok] - b[ok]).max()
 
     near(got[0], lp, tol)
     near(got[1], ent, tol * (1 + np.where(np.isnan(ent), 0, ent)))
@@ -83,6 +83,16 @@ def test_device_token_ids_are_checked_on_the_host():
     for bad in ({"typestr": "<i8"}, {"strides": (8,)}, {"shape": (2, 2), "strides": (16, 4)}):
         with pytest.raises(ValueError, match="32-bit"):
             tb.LogProbs._tokens(Array(**bad))
+
+
+def test_host_token_ids_are_checked_and_copied():
+    for bad in ([-1], [2 ** 32], [1.5], np.array([3, 2 ** 32 + 5])):
+        with pytest.raises(ValueError, match="32 bits"):
+            tb.LogProbs._tokens(bad)
+    assert tb.LogProbs._tokens([])[1] == 0
+    given = np.array([4, 2 ** 32 - 1], dtype=np.uint32)
+    ptr, n, kept = tb.LogProbs._tokens(given)
+    assert n == 2 and kept.tolist() == given.tolist() and ptr != given.ctypes.data
 
 
 @pytest.mark.gpu
@@ -179,6 +189,83 @@ def test_many_rows_of_every_alignment(b200, top):
     compare(got, x, tokens, top)
     for a, c in zip(got, s.score(b, tokens)):
         assert np.array_equal(a.view(np.int32), c.view(np.int32))
+
+
+def row_kinds(vocab):
+    """Rows of nine kinds, the alternatives spread, side by side, at either end, tied."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((9, vocab)).astype(F32) * F32(2)
+    x[1] = np.round(x[1])
+    x[2] = F32(0.5)  # every logit the same
+    x[3] = np.sort(x[3])
+    x[4] = np.sort(x[4])[::-1]
+    x[5, vocab // 2:vocab // 2 + 300] += F32(12)
+    x[6, rng.integers(0, vocab, 4)] += F32(25)
+    x[7, rng.permutation(vocab)[vocab // 100:]] = -np.inf  # few are left, perhaps fewer than the alternatives
+    x[8] = np.where(np.arange(vocab) % 128 < 40, x[8], x[8] - F32(30))
+    return x
+
+
+# Rows by a warp each in registers or step by step, by a CTA each, in pieces, in
+# runs that end inside rows; one warp's share of a row is at most 64 steps of 16.
+MANY_ROWS = [(9, 2045, 64), (1300, 2045, 7), (126, 2046, 64), (126, 2046, 2), (333, 2051, 0), (333, 2051, 1),
+             (700, 5003, 1), (300, 5003, 20), (900, 16381, 40), (4200, 32765, 0), (1650, 32765, 5), (400, 32765, 5),
+             (64, 32001, 0), (64, 32001, 5), (100, 33001, 1), (1, 20001, 3), (400, 40003, 3), (650, 40003, 0),
+             (650, 40003, 1), (650, 40003, 6), (250, 300007, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,top", MANY_ROWS)
+def test_ways_of_sharing_rows(b200, rows, vocab, top):
+    torch = pytest.importorskip("torch")
+    x = row_kinds(vocab)
+    tokens = np.array([0, vocab - 1, 5, vocab - 1, 0, vocab // 2, 7, 8, 1])
+    at = np.arange(rows) % 9
+    b = b200.alloc(rows * vocab)
+    given = torch.as_tensor(x, device="cuda")[torch.as_tensor(at, device="cuda")]
+    torch.as_tensor(b, device="cuda").copy_(given.reshape(-1))
+    torch.cuda.synchronize()
+    got = tb.LogProbs(b200, rows, vocab, top).score(b, tokens[at])
+    for first in {0, (rows - 1) // 18 * 9, (rows - 1) // 9 * 9}:
+        part = slice(first, min(first + 9, rows))
+        n = part.stop - part.start
+        compare([g[part] for g in got], x[:n], tokens[:n], top)
+    # Each row's alternatives whatever its place; its sums to twice the tolerance above, a span of 100 taken for all.
+    for i in range(min(9, rows)):
+        assert (got[2][i::9] == got[2][i]).all()
+        for g in (got[0], got[1]):
+            assert np.array_equal(np.isfinite(g[i::9]), np.full(len(g[i::9]), np.isfinite(g[i])))
+            if np.isfinite(g[i]):
+                assert np.abs(g[i::9] - g[i]).max() <= 2 * (CHAIN + 400) * EPS * (1 + abs(g[i]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,top", [(2101, 0), (2101, 1), (2101, 33), (9001, 5), (9001, 64)])
+def test_many_rows_that_are_not_ordinary(b200, vocab, top):
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((10, vocab)).astype(F32)
+    x[0, : vocab // 2] = -np.inf
+    x[1] = -np.inf
+    x[2], x[2, 17] = -np.inf, 3.0
+    x[3, vocab - 1] = np.nan
+    x[4, 6] = np.inf
+    x[5, 9] = -np.float32(np.nan)
+    x[6] = np.where(np.arange(vocab) % 3 == 0, F32(0.0), F32(-0.0))
+    x[7] = np.finfo(F32).min
+    x[8], x[8, 4], x[8, 5] = np.finfo(F32).max, 0.0, np.finfo(F32).min
+    x[9, 1:] = -np.inf
+    rows = 1260
+    at = np.arange(rows) % 10
+    many = x[at]
+    got = tb.LogProbs(b200, rows, vocab, top).score(buf(b200, many), at * 3)
+    lp, ent, ids, tops = reference(x, np.arange(10) * 3, top)
+    assert (got[2] == ids[at]).all()
+    for g, e in ((got[0], lp), (got[1], ent), (got[3], tops)):
+        e = e[at]
+        assert np.array_equal(np.isnan(g), np.isnan(e))
+        assert np.array_equal(np.isneginf(g), np.isneginf(e))
+        ok = np.isfinite(e)
+        assert np.all(np.abs(g[ok] - e[ok]) <= CHAIN * EPS * (2 + np.abs(e[ok])))
 
 
 @pytest.mark.gpu

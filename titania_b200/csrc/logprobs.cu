@@ -11,27 +11,28 @@
 // Both terms of the entropy are positive and log1p keeps S's relative error,
 // so neither loses digits when one token has almost all of the probability.
 //
-// One pass over the logits, bound by reading them (1111 x 151936: 110 us, of
-// which the bytes take 105). The rows' steps of 512 logits, one after another, are
-// dealt out to the CTAs that run at once in equal runs (whatever the number of
-// rows, no SM waits for another's last one); a CTA's part of a row is a piece. A
-// warp takes a step at a time, as four blocks of 128: their largest, a redux each,
-// are both the running maximum that the sums refer to and the blocks' entries in
-// a table of 1/128 of the logits' size. The warps of a CTA begin a piece with the
-// largest of their first steps as common maximum, so that few steps raise it:
-// that is a warp-uniform branch as dear as a step. Per logit there are five
-// instructions for the sums and one for the maximum; at ten the kernel was bound
-// by them (142 us). The CTA that finishes a row's last piece joins the pieces'
-// sums, in their order.
+// One pass over the logits, in steps of 512 of a row, which a warp takes at a time as four blocks of 128. The
+// blocks' largest, a redux each, are both the running maximum that the sums refer
+// to and their entries in a table of 1/128 of the logits' size. Per logit there
+// are five instructions for the sums and one for the maximum; at ten the kernel
+// was bound by them (1111 x 151936: 142 us; 108, of which the bytes take 105). Who takes what:
+//   k_score_rows       rows of up to four steps: a warp a row, in its registers;
+//   k_score_long_rows  many rows of up to 64 steps: a warp a row, step by step;
+//   k_score            else: a CTA a row, or a part of one (deal() below). The CTA
+//                      that finishes a row's last piece joins the pieces' sums, in
+//                      their order.
+// The warps of a CTA begin a piece with the largest of their first steps as
+// common maximum, so that few steps raise it: that is a warp-uniform branch as
+// dear as a step.
 //
 // The alternatives: the k largest logits lie in the k blocks with the largest
 // maxima (each of those has an element at least as large as any element of
-// another block), so only those are read again. That is a few microseconds a row,
-// of waiting more than of work: with few rows the CTA that finishes a row does it
-// (64 rows, five alternatives: 16 us, 11.5 with none), with many it is a kernel of
-// its own with a CTA for every row (1111 rows: 125 us; in one kernel 131). One warp
-// alone takes 20 us for it. One alternative is the maximum itself, whose place
-// the warps keep (117 us).
+// another block), so only those are read again. In k_score that is a few
+// microseconds a row, of waiting more than of work: with few rows the CTA that
+// finishes a row does it (64 rows, five alternatives: 15.8 us, 11.5 with none),
+// with many it is a kernel of its own with a CTA for every row (1111 rows: 124 us;
+// in one kernel 131). One alternative is the maximum itself, whose place the warps
+// keep (112 us).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -188,10 +189,10 @@ struct Running {
 
 // The largest in order of each of four blocks, for the warp; the largest of
 // them. `real(u, j)`: value j of block u is the row's (`whole`: all are). nan:
-// set to a NaN that a lane meets.
+// set to a NaN that a lane meets. lane_top: raised to the lane's own largest of each block.
 template <class Real>
 __device__ __forceinline__ int step_max(const float (&x)[kStep][4], int (&bm)[kStep], float& nan, bool whole,
-                                        Real real) {
+                                        Real real, int* lane_top = nullptr) {
   float m[kStep], least = INFINITY;
 #pragma unroll
   for (int u = 0; u < kStep; u++) {
@@ -215,6 +216,9 @@ __device__ __forceinline__ int step_max(const float (&x)[kStep][4], int (&bm)[kS
       }
     }
   }
+  if (lane_top)
+#pragma unroll
+    for (int u = 0; u < kStep; u++) lane_top[u] = max(lane_top[u], bm[u]);
   __syncwarp();
 #pragma unroll
   for (int u = 0; u < kStep; u++) bm[u] = __reduce_max_sync(0xffffffffu, bm[u]);
@@ -277,7 +281,8 @@ struct ScoreArgs {
   float2* peak;     // [rows] maximum and log Z for k_alternatives
   int vocab, top;
   int steps;        // of a row, whatever its alignment
-  long long total;  // steps of all rows
+  int pitch;        // of a row where they are dealt out: steps, or a multiple of run
+  long long total;  // rows * pitch
   long long run;    // steps of a CTA
 };
 
@@ -505,9 +510,10 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
   long long g = blockIdx.x * a.run;
   const long long g1 = min(a.total, g + a.run);
   while (g < g1) {
-    const size_t row = size_t(g / a.steps);
-    const int s0 = int(g - (long long)row * a.steps), s1 = int(min((long long)a.steps, s0 + (g1 - g)));
-    g += s1 - s0;
+    const size_t row = size_t(g / a.pitch);
+    const int s0 = int(g - (long long)row * a.pitch), end = int(min((long long)a.pitch, s0 + (g1 - g)));
+    const int s1 = min(end, a.steps);
+    g += end - s0;
     const Row r(a.logits, row, a.vocab);
     int* block_max = TOP != kTopOne && a.block_max ? a.block_max + row * size_t(a.steps) * kStep : nullptr;
     // The token's logit, for whoever finishes the row: on its way while the others are read.
@@ -575,7 +581,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     if (TOP == kTopOne) best = warp_umax64(sh.best[lane % kScoreWarps]);
     // Pieces of this row: those of the CTAs whose runs meet it.
     int entry[kOwn];
-    const long long c0 = (long long)row * a.steps / a.run, c1 = ((long long)(row + 1) * a.steps - 1) / a.run;
+    const long long c0 = (long long)row * a.pitch / a.run, c1 = ((long long)(row + 1) * a.pitch - 1) / a.run;
     if (c1 > c0) {
       if (threadIdx.x == 0) {
         a.part[row + blockIdx.x] = make_float4(s.m, s.s, s.t, s.own);
@@ -772,8 +778,201 @@ __global__ void __launch_bounds__(kScoreThreads) k_score_rows(ScoreArgs a, int r
   }
 }
 
+// Rows of up to kRowSteps steps where there are enough of them: a warp each again,
+// which goes through its row and has the next step on its way meanwhile. For
+// the alternatives the row falls into 128 sets, each lane's places in the four
+// blocks of every step: k of the sets' largest logits are at least the k-th of
+// them, which bounds the k-th logit from below closely (about 1.4 k logits reach it at
+// k = 64). The blocks that reach it, by their maxima, are read again. 2048 x 5000, us,
+// no and twenty alternatives: 10.2 and 19.7, by k_score and k_alternatives 17.2 and 48.1.
+constexpr int kRowSteps = 64;
+constexpr int kRowWarps = 4;
+constexpr int kRoom = 256;  // candidates that a warp holds
+static_assert(kRoom >= kPicked + kBlock, "after a cut there is room for a block");
+__global__ void __launch_bounds__(32 * kRowWarps) k_score_long_rows(ScoreArgs a, int rows) {
+  __shared__ int4 tables[kRowWarps][kRowSteps];
+  __shared__ unsigned long long rooms[kRowWarps][kRoom];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * kRowWarps + warp;
+  if (row >= rows) return;
+  const Row r(a.logits, size_t(row), a.vocab);
+  const float nan = __int_as_float(0x7FC00000);
+  const uint32_t tok = a.tokens[row];
+  const float given = tok < uint32_t(a.vocab) ? __ldg(r.base + r.shift + tok) : nan;
+  auto whole = [&](int st) { return r.inside(st * kStep) && r.inside(st * kStep + kStep - 1); };
+  auto fetch = [&](int st, float4 (&v)[kStep]) {
+    const bool w = whole(st);
+#pragma unroll
+    for (int u = 0; u < kStep; u++) {
+      const int b = st * kStep + u;
+      v[u] = w ? r.load(b, lane) : r.load_end(b, lane, -INFINITY);
+    }
+  };
+  float met = 0.f;
+  int sets[kStep] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
+  Running run(kNegInf);
+  float4 next[kStep];
+  fetch(0, next);
+#pragma unroll 2
+  for (int st = 0; st < a.steps; st++) {
+    float x[kStep][4];
+#pragma unroll
+    for (int u = 0; u < kStep; u++) x[u][0] = next[u].x, x[u][1] = next[u].y, x[u][2] = next[u].z, x[u][3] = next[u].w;
+    if (st + 1 < a.steps) fetch(st + 1, next);
+    int bm[kStep];
+    const bool w = whole(st);
+    const int top = step_max(x, bm, met, w, [&](int u, int j) {
+      const int at = r.element(st * kStep + u, lane, j);
+      return w || (at >= 0 && at < a.vocab);
+    }, sets);
+    if (lane == 0) tables[warp][st] = make_int4(bm[0], bm[1], bm[2], bm[3]);
+    const bool higher = top > run.order;
+    if (higher) run.raise(top, lane);
+    step_add(run, x, lane, higher);
+  }
+  run.s += met * 0.0f;  // a NaN stays
+  Soft f = run.settled();
+  f.s = warp_sum(f.s);
+  f.t = warp_sum(f.t);
+  const bool bad = !(f.m < INFINITY) || f.m == -INFINITY || isnan(f.s);
+  const float logz = bad ? nan : log1pf(f.s);
+  if (lane == 0) {
+    a.entropy[row] = logz + kLn2 * f.t / (1.0f + f.s);
+    a.logprob[row] = (given - f.m) - logz;
+  }
+  const int k = a.top;
+  if (!k) return;
+  // From here on no key below `least` is among the k largest.
+  unsigned long long least;
+  unsigned own[kStep], hi;
+  {
+#pragma unroll
+    for (int u = 0; u < kStep; u++) own[u] = unsigned(sets[u]) ^ 0x80000000u;
+    const unsigned high = max(max(own[0], own[1]), max(own[2], own[3]));
+    hi = __reduce_max_sync(0xffffffffu, high);
+    unsigned lo = hi;
+    if (k > 1) {
+      lo = __reduce_min_sync(0xffffffffu, k <= 32 ? high : min(min(own[0], own[1]), min(own[2], own[3])));
+      for (unsigned top = hi; lo < top;) {  // lo: reached by k sets at least
+        const unsigned mid = lo + (top - lo) / 2 + 1;
+        const int c =
+            __reduce_add_sync(0xffffffffu, (own[0] >= mid) + (own[1] >= mid) + (own[2] >= mid) + (own[3] >= mid));
+        if (c >= k) {
+          lo = mid;
+          if (c <= k + k / 8) break;
+        } else {
+          top = mid - 1;
+        }
+      }
+    }
+    least = max(1ull, static_cast<unsigned long long>(lo) << 32);
+  }
+  const unsigned long long most = (static_cast<unsigned long long>(hi) << 32) | 0xFFFFFFFFull;
+  unsigned long long* room = rooms[warp];
+  int n = 0;
+  // Cuts the candidates down to slack(k), where rows rise or have many equal logits.
+  auto cut = [&] {
+    unsigned long long mine[kRoom / 32];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kRoom / 32; i++) mine[i] = i * 32 + lane < n ? room[i * 32 + lane] : 0ull;
+    least = key_bound(k, slack(k), least, most, [&](unsigned long long key) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < kRoom / 32; i++) c += mine[i] >= key;
+      return __reduce_add_sync(0xffffffffu, c);
+    });
+    __syncwarp();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < kRoom / 32; i++) {
+      const unsigned who = __ballot_sync(0xffffffffu, mine[i] >= least);
+      if (mine[i] >= least) room[n + __popc(who & ((1u << lane) - 1))] = mine[i];
+      n += __popc(who);
+    }
+  };
+  const int* table = reinterpret_cast<const int*>(tables[warp]);
+  __syncwarp();
+  for (int b0 = 0; b0 < r.blocks; b0 += 32) {
+    const int b = b0 + lane;
+    unsigned picked = __ballot_sync(0xffffffffu, b < r.blocks && order_key(table[min(b, r.blocks - 1)], 0) >= least);
+    while (picked) {
+      constexpr int kBatch = 4;
+      float4 v[kBatch];
+      int bs[kBatch], m = 0;
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        if (!picked) break;
+        bs[i] = b0 + __ffs(picked) - 1;
+        picked &= picked - 1;
+        v[i] = r.inside(bs[i]) ? r.load(bs[i], lane) : r.load_end(bs[i], lane, 0.f);
+        m = i + 1;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        if (i >= m) break;
+        if (n + kBlock > kRoom) cut();
+        const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int o = order(x[j]);
+          if (!__any_sync(0xffffffffu, (unsigned(o) ^ 0x80000000u) >= unsigned(least >> 32))) continue;
+          const int at = r.element(bs[i], lane, j);
+          const unsigned long long key = at >= 0 && at < r.vocab ? order_key(o, uint32_t(at)) : 0ull;
+          const unsigned who = __ballot_sync(0xffffffffu, key >= least);
+          if (key >= least) room[n + __popc(who & ((1u << lane) - 1))] = key;
+          n += __popc(who);
+        }
+      }
+    }
+  }
+  if (n > kPicked) cut();
+  __syncwarp();
+  // Each candidate's rank: a lane's up to four at once, against all.
+  constexpr int kMine = (kPicked + 31) / 32;
+  unsigned long long mine[kMine];
+  int rank[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++) mine[i] = i * 32 + lane < n ? room[i * 32 + lane] : 0ull, rank[i] = 0;
+  for (int j = 0; j < n; j++) {
+    const unsigned long long other = room[j];
+#pragma unroll
+    for (int i = 0; i < kMine; i++)
+      if (i * 32 < n) rank[i] += other > mine[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; i++)
+    if (mine[i] && rank[i] < k) {
+      a.top_ids[row * k + rank[i]] = argmax_index(mine[i]);
+      a.top_logprobs[row * k + rank[i]] = (unorder(int(uint32_t(mine[i] >> 32) ^ 0x80000000u)) - f.m) - logz;
+    }
+}
+
 // Steps of a row, whatever its alignment.
 int score_steps(size_t vocab) { return int((vocab + 3 + kStep * kBlock - 1) / (kStep * kBlock)); }
+
+// How k_score's CTAs share the rows: a row each; each row cut into equal pieces, a
+// CTA for each; or all rows' steps in equal runs for the CTAs that run at once. By the steps
+// of the CTA that has most, a join counted as 32 and two pieces for a CTA as 64 (us, without alternatives:
+// 1 x 5000 4.1 whole and 5.1 cut, 1 x 32000 7.1 and 5.5; 64 x 32000 7.8 whole, 11.4 in equal runs,
+// 7.2 in pieces; 2048 x 32000 51.9 whole and 55.3 in runs).
+void deal(ScoreArgs& a, long long n, long long ctas) {
+  const long long whole = (n + ctas - 1) / ctas * a.steps;
+  const long long even = std::max<long long>((n * a.steps + ctas - 1) / ctas, std::min(a.steps, kScoreWarps));
+  const long long each = std::max<long long>(1, ctas / n);  // pieces of a row
+  const long long piece = std::max<long long>((a.steps + each - 1) / each, std::min(a.steps, kScoreWarps));
+  a.run = a.pitch = a.steps;
+  long long least = whole;
+  if (piece < a.steps && piece + 32 < least) {
+    least = piece + 32;
+    a.run = piece;
+    a.pitch = int((a.steps + piece - 1) / piece * piece);
+  }
+  if (even + 64 < least) a.run = even, a.pitch = a.steps;
+  a.total = n * a.pitch;
+}
 
 }  // namespace
 }  // namespace tb
@@ -899,9 +1098,7 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
   a.vocab = int(s->vocab);
   a.top = s->top;
   a.steps = tb::score_steps(s->vocab);
-  a.total = (long long)n * a.steps;
-  // Equal runs for the CTAs that run at once, of a step for every warp at least where rows are that long.
-  a.run = std::max<long long>((a.total + s->ctas - 1) / s->ctas, std::min(a.steps, tb::kScoreWarps));
+  tb::deal(a, (long long)n, s->ctas);
   a.part_best = s->part_best;
   a.peak = s->peak;
   const dim3 grid(unsigned((a.total + a.run - 1) / a.run)), block(tb::kScoreThreads);
@@ -913,6 +1110,12 @@ int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint3
       tb::launch_pdl(tb::k_score_rows<2>, warps, block, 0, st, a, int(n));
     else
       tb::launch_pdl(tb::k_score_rows<4>, warps, block, 0, st, a, int(n));
+  } else if (a.steps <= tb::kRowSteps && n > size_t(s->top > 1 ? 25 : 64) * a.steps) {
+    // Enough rows that warps which go through theirs alone fill the GPU (us there and with a CTA a row: no
+    // alternatives, 800 x 2100 5.8 and 6.5, 256 x 2100 4.6 and 4.2, 800 x 16000 21 and 12.5; five, 256 x 5000 9.6
+    // and 12.5, 2048 x 32000 63 and 78, 800 x 32000 49 and 37).
+    tb::launch_pdl(tb::k_score_long_rows, dim3(unsigned((n + tb::kRowWarps - 1) / tb::kRowWarps)),
+                   dim3(32 * tb::kRowWarps), 0, st, a, int(n));
   } else if (s->top == 1) {
     tb::launch_pdl(tb::k_score<tb::kTopOne>, grid, block, 0, st, a);
   } else if (s->top && 2 * n <= size_t(s->ctas)) {

@@ -629,7 +629,10 @@ class LogProbs:
         the CUDA array interface, 32-bit integers) or on the host."""
         a = getattr(tokens, "__cuda_array_interface__", None)
         if a is None:
-            t = np.ascontiguousarray(tokens, dtype=np.uint32).reshape(-1)
+            t = np.asarray(tokens).reshape(-1)
+            if t.size and (t.dtype.kind not in "iu" or t.min() < 0 or t.max() > 0xFFFFFFFF):
+                raise ValueError("token ids must be integers of 32 bits")
+            t = np.array(t, dtype=np.uint32)  # in pageable memory, which the call copies before it returns
             return t.ctypes.data, t.size, t
         n = math.prod(a["shape"])
         if a["typestr"] not in ("<i4", "<u4") or (a.get("strides") and n > 1 and (
