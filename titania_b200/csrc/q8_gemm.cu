@@ -406,44 +406,44 @@ __global__ void __launch_bounds__(kQThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-        // Epilogue warps: scales and writes the sums of 32 tokens (quarter q of the
+  // Epilogue warps: scales and writes the sums of 32 tokens (quarter q of the
   // tile at m0) by up to 32 channels from column c of the tile at n0, a lane a
   // token, through this warp's staging tile, where 16-byte piece j of a row
   // lies at j ^ (row & 7). b: which of tl.sw.
   unsigned char* tile_s = staging + (warp - 2) * kStageTile;
   float4* mine_s = reinterpret_cast<float4*>(tile_s + lane * 128);
-        auto put = [&](int b, int m0, int n0, int q, int c, float sx, int (&acc)[32]) {
-      const int cols = min(n, a.M - n0);
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile's last store
-          __syncwarp();
-          const bool half = c + 32 > n;  // the tile ends after 16 channels: rows of 64 bytes, not swizzled
-          float4* to_s = half ? reinterpret_cast<float4*>(tile_s + lane * 64) : mine_s;
-          const int flip = half ? 0 : lane & 7;
-  #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            if (half && j >= 4) break;
-            const float4 sw = *reinterpret_cast<const float4*>(&tl.sw[b][c + 4 * j]);
-            to_s[j ^ flip] = make_float4(__fmul_rn(__int2float_rn(acc[4 * j]), __fmul_rn(sw.x, sx)),
-                                         __fmul_rn(__int2float_rn(acc[4 * j + 1]), __fmul_rn(sw.y, sx)),
-                                         __fmul_rn(__int2float_rn(acc[4 * j + 2]), __fmul_rn(sw.z, sx)),
-                                         __fmul_rn(__int2float_rn(acc[4 * j + 3]), __fmul_rn(sw.w, sx)));
-          }
-          if (a.tma_out) fence_proxy_async_smem();
-          __syncwarp();
-          if (a.tma_out) {
-            if (lane == 0) {
-              tma_store_2d(half ? &tout16 : &tout, n0 + c, m0 + 32 * q, tile_s);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else if (c + lane < cols) {
-            const int rows = min(32, a.T - m0 - 32 * q), pitch = half ? 64 : 128;
-            float* to = a.out + size_t(m0 + 32 * q) * a.M + n0 + c + lane;
-            for (int r = 0; r < rows; r++, to += a.M)
-              *to = *reinterpret_cast<const float*>(tile_s + r * pitch + (((lane >> 2) ^ (half ? 0 : r & 7)) << 4) +
-                                                    (lane & 3) * 4);
-          }
-          __syncwarp();
-        };
+  auto put = [&](int b, int m0, int n0, int q, int c, float sx, int (&acc)[32]) {
+    const int cols = min(n, a.M - n0);
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile's last store
+    __syncwarp();
+    const bool half = c + 32 > n;  // the tile ends after 16 channels: rows of 64 bytes, not swizzled
+    float4* to_s = half ? reinterpret_cast<float4*>(tile_s + lane * 64) : mine_s;
+    const int flip = half ? 0 : lane & 7;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (half && j >= 4) break;
+      const float4 sw = *reinterpret_cast<const float4*>(&tl.sw[b][c + 4 * j]);
+      to_s[j ^ flip] = make_float4(__fmul_rn(__int2float_rn(acc[4 * j]), __fmul_rn(sw.x, sx)),
+                                   __fmul_rn(__int2float_rn(acc[4 * j + 1]), __fmul_rn(sw.y, sx)),
+                                   __fmul_rn(__int2float_rn(acc[4 * j + 2]), __fmul_rn(sw.z, sx)),
+                                   __fmul_rn(__int2float_rn(acc[4 * j + 3]), __fmul_rn(sw.w, sx)));
+    }
+    if (a.tma_out) fence_proxy_async_smem();
+    __syncwarp();
+    if (a.tma_out) {
+      if (lane == 0) {
+        tma_store_2d(half ? &tout16 : &tout, n0 + c, m0 + 32 * q, tile_s);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else if (c + lane < cols) {
+      const int rows = min(32, a.T - m0 - 32 * q), pitch = half ? 64 : 128;
+      float* to = a.out + size_t(m0 + 32 * q) * a.M + n0 + c + lane;
+      for (int r = 0; r < rows; r++, to += a.M)
+        *to = *reinterpret_cast<const float*>(tile_s + r * pitch + (((lane >> 2) ^ (half ? 0 : r & 7)) << 4) +
+                                              (lane & 3) * 4);
+    }
+    __syncwarp();
+  };
 
   // The producer's and the MMA warp's lanes stay together and one of them is
   // elected at each instruction: what they issue takes uniform registers, and
