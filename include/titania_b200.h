@@ -188,7 +188,8 @@ TB200_API int tb200_silu_mul(tb200_device* dev, tb200_buffer* gate, const tb200_
  * multiplies the two. Everything below is enqueued on the device's stream and
  * returns without waiting, unless it says otherwise; no call but the ones
  * that make a handle allocates memory, so calls can be captured into a CUDA
- * graph on that stream. A call with no rows does nothing.
+ * graph on that stream. A call with no rows does nothing. All handles of a
+ * call were made on its device.
  *
  * How values become integers, everywhere here: with m the largest magnitude
  * of a row's values, the scale is m / 127 rounded to f32, and each integer is

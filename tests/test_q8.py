@@ -220,7 +220,8 @@ def test_resized_rows(b200):
 
 PRODUCTS = [
     # tokens, channels, columns
-    (3, 17000, 2600), (4, 40001, 1100), (1, 1, 1), (1, 5, 16), (1, 4096, 1024), (1, 33, 1001), (1, 1000, 10240), (2, 128, 128), (3, 257, 96), (4, 9, 2560),
+    (3, 17000, 2600), (4, 40001, 1100), (1, 1, 1), (1, 5, 16), (1, 4096, 1024), (1, 33, 1001), (1, 1000, 10240),
+    (2, 128, 128), (3, 257, 96), (4, 9, 2560),
     (5, 300, 130), (7, 131, 777), (8, 1024, 512), (9, 640, 2560), (15, 40, 3000), (16, 128, 64), (17, 129, 1001),
     (31, 1000, 31), (33, 77, 4100), (48, 4096, 1024), (63, 2560, 96), (64, 640, 2560), (65, 130, 200), (100, 1, 100),
     (128, 1024, 1024), (129, 513, 640), (200, 2560, 257), (256, 256, 9728), (300, 1200, 1100), (511, 1023, 511),
@@ -359,6 +360,28 @@ def test_calls_with_no_rows(b200):
     assert [a.shape for a in b200.read_q8(q)] == [(0, 64), (0,)]
     b200.write_q8(q, np.zeros((0, 64), np.int8), np.zeros(0, F32))
     assert b200.quantize_weight(b200.upload(tb.Tensor([0, 64], np.zeros(0, np.uint16)))).shape == (0, 64)
+
+
+@pytest.mark.gpu
+def test_operands_of_another_device(b200):
+    """Refused before anything is launched; here another device is another handle of the same GPU."""
+    other = tb.B200(0)
+    bits = np.full((4, 64), 0x3F80, np.uint16)
+    q, x, w = b200.q8(4, 64), b200.alloc(256), b200.upload(tb.Tensor([64], bits[0]))
+    m = b200.upload(tb.Tensor([4, 64], bits))
+    q2, x2, w2, out = other.q8(4, 64), other.alloc(256), other.upload(tb.Tensor([64], bits[0])), b200.alloc(16)
+    for call in (lambda: b200.quantize(q2, x), lambda: b200.quantize(q, x2), lambda: b200.dequantize(x2, q),
+                 lambda: b200.dequantize(x, q2), lambda: b200.add_rmsnorm_q8(q2, x, None, w, 1e-6),
+                 lambda: b200.add_rmsnorm_q8(q, x2, None, w, 1e-6), lambda: b200.add_rmsnorm_q8(q, x, x2, w, 1e-6),
+                 lambda: b200.add_rmsnorm_q8(q, x, None, w2, 1e-6), lambda: b200.matmul_q8(out, q2, q),
+                 lambda: b200.matmul_q8(out, q, q2), lambda: b200.matmul_q8(x2, q, q), lambda: other.quantize_weight(m),
+                 lambda: b200.read_q8(q2), lambda: b200.resize_q8(q2, 2),
+                 lambda: b200.write_q8(q2, np.zeros((4, 64), np.int8), np.zeros(4, F32)),
+                 lambda: tb.LogProbs(b200, 4, 64).score(x2, [0])):
+        with pytest.raises(tb.DeviceError, match="another device"):
+            call()
+    other.sync()
+    b200.sync()
 
 
 # ---- with torch, and captured --------------------------------------------------------------

@@ -463,6 +463,7 @@ int upload_impl(tb200_device* d, const char* path, const char* const* names, con
   for (size_t i = 0; i < n; i++) {
     if (!ent[i]) continue;
     auto* w = new tb200_weight;
+    w->dev = d;
     const bool whole = !win || (win[i].rows == 0 && win[i].cols == 0);
     w->shape = whole ? ent[i]->shape : std::vector<size_t>{win[i].rows, win[i].cols};
     w->numel = numel[i];

@@ -1065,6 +1065,7 @@ int tb200_scorer_free(tb200_scorer* s) {
 
 int tb200_score_enqueue(tb200_scorer* s, const tb200_buffer* logits, const uint32_t* tokens, size_t n) {
   ARG_CHECK(s && logits && (tokens || !n), "null argument");
+  ARG_CHECK(rt::of(s->dev, logits), "score: the logits were made on another device than the scorer");
   ARG_CHECK(n <= s->rows, "score: a scorer of " + std::to_string(s->rows) + " rows can't hold " + std::to_string(n));
   ARG_CHECK(logits->len >= n * s->vocab, "score: the logits buffer holds fewer than rows x vocabulary values");
   if (int rc = rt::use(s->dev)) return rc;

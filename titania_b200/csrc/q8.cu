@@ -431,6 +431,7 @@ int tb200_q8_new(tb200_device* d, size_t rows, size_t cols, tb200_q8** out) {
   ARG_CHECK(cols > 0 && cols <= kMaxDim, "q8: bad number of columns");
   ARG_CHECK(rows <= kMaxDim, "q8: too many rows");
   auto* q = new tb200_q8;
+  q->dev = d;
   q->rows = q->cap = rows;
   q->cols = cols;
   q->ld = (cols + 15) / 16 * 16;
@@ -452,6 +453,7 @@ int tb200_q8_new(tb200_device* d, size_t rows, size_t cols, tb200_q8** out) {
 int tb200_q8_free(tb200_device* d, tb200_q8* q) {
   if (!q) return TB200_OK;
   if (int rc = rt::use(d)) return rc;
+  ARG_CHECK(rt::of(d, q), "free: the 8-bit rows were made on another device");
   CUDA_TRY(cudaStreamSynchronize(d->stream));
   q8_release(q);
   return TB200_OK;
@@ -460,6 +462,7 @@ int tb200_q8_free(tb200_device* d, tb200_q8* q) {
 int tb200_q8_resize(tb200_device* d, tb200_q8* q, size_t rows) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(q, "null argument");
+  ARG_CHECK(rt::of(d, q), "resize: the 8-bit rows were made on another device");
   ARG_CHECK(rows <= q->cap, "8-bit rows made for " + std::to_string(q->cap) + " can't hold " + std::to_string(rows));
   q->rows = rows;
   return TB200_OK;
@@ -475,6 +478,7 @@ int tb200_q8_shape(const tb200_q8* q, size_t* rows, size_t* cols) {
 int tb200_q8_read(tb200_device* d, const tb200_q8* q, int8_t* values, float* scales) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(q && ((values && scales) || !q->rows), "null argument");
+  ARG_CHECK(rt::of(d, q), "the 8-bit rows were made on another device");
   if (q->rows) {
     CUDA_TRY(cudaMemcpy2DAsync(values, q->cols, q->values, q->ld, q->cols, q->rows, cudaMemcpyDeviceToHost, d->stream));
     CUDA_TRY(cudaMemcpyAsync(scales, q->scales, q->rows * 4, cudaMemcpyDeviceToHost, d->stream));
@@ -485,6 +489,7 @@ int tb200_q8_read(tb200_device* d, const tb200_q8* q, int8_t* values, float* sca
 int tb200_q8_write(tb200_device* d, tb200_q8* q, const int8_t* values, const float* scales) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(q && ((values && scales) || !q->rows), "null argument");
+  ARG_CHECK(rt::of(d, q), "the 8-bit rows were made on another device");
   if (q->rows) {
     CUDA_TRY(cudaMemcpy2DAsync(q->values, q->ld, values, q->cols, q->cols, q->rows, cudaMemcpyHostToDevice, d->stream));
     CUDA_TRY(cudaMemcpyAsync(q->scales, scales, q->rows * 4, cudaMemcpyHostToDevice, d->stream));
@@ -503,6 +508,7 @@ int tb200_q8_data(const tb200_q8* q, int8_t** values, size_t* ld, float** scales
 int tb200_quantize(tb200_device* d, tb200_q8* out, const tb200_buffer* x) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(out && x, "null argument");
+  ARG_CHECK(rt::of(d, out, x), "quantize: an operand was made on another device");
   ARG_CHECK(x->len == out->rows * out->cols, "quantize: input holds " + std::to_string(x->len) + " values, expected " +
                                                  std::to_string(out->rows * out->cols));
   if (!out->rows) return TB200_OK;
@@ -515,6 +521,7 @@ int tb200_quantize(tb200_device* d, tb200_q8* out, const tb200_buffer* x) {
 int tb200_quantize_weight(tb200_device* d, const tb200_weight* w, tb200_q8** out) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(w && out, "null argument");
+  ARG_CHECK(rt::of(d, w), "quantize_weight: the weight was made on another device");
   ARG_CHECK(w->shape.size() == 2, "quantize_weight: weight is not a matrix");
   tb200_q8* q = nullptr;
   if (int rc = tb200_q8_new(d, w->shape[0], w->shape[1], &q)) return rc;
@@ -534,6 +541,7 @@ int tb200_quantize_weight(tb200_device* d, const tb200_weight* w, tb200_q8** out
 int tb200_dequantize(tb200_device* d, tb200_buffer* out, const tb200_q8* x) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(out && x, "null argument");
+  ARG_CHECK(rt::of(d, out, x), "dequantize: an operand was made on another device");
   ARG_CHECK(out->len == x->rows * x->cols, "dequantize: output holds " + std::to_string(out->len) +
                                                " values, expected " + std::to_string(x->rows * x->cols));
   if (!x->rows) return TB200_OK;
@@ -554,6 +562,7 @@ int tb200_add_rmsnorm_q8(tb200_device* d, tb200_q8* out, tb200_buffer* x, const 
                          const tb200_weight* w, float eps) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(out && x && w, "null argument");
+  ARG_CHECK(rt::of(d, out, x, y, w), "add_rmsnorm_q8: an operand was made on another device");
   ARG_CHECK(x != y, "add_rmsnorm_q8: x and y are the same buffer");
   const size_t n = out->rows * out->cols;
   ARG_CHECK(x->len == n, "add_rmsnorm_q8: x holds " + std::to_string(x->len) + " values, expected " + std::to_string(n));

@@ -785,6 +785,7 @@ extern "C" {
 int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const tb200_q8* x) {
   if (int rc = rt::use(d)) return rc;
   ARG_CHECK(out && w && x, "null argument");
+  ARG_CHECK(rt::of(d, out, w, x), "matmul_q8: an operand was made on another device");
   ARG_CHECK(w->cols == x->cols, "matmul_q8: weight has " + std::to_string(w->cols) + " columns, input " +
                                     std::to_string(x->cols));
   ARG_CHECK(w->cols <= tb::kMaxCols, "matmul_q8: more than 131071 columns do not sum in 32 bits");

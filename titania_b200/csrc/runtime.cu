@@ -222,6 +222,7 @@ int tb200_upload(tb200_device* d, const uint16_t* data, const size_t* shape, siz
   if (int rc = use(d)) return rc;
   ARG_CHECK(out && (data || ndim == 0) && (shape || ndim == 0), "null argument");
   auto* w = new tb200_weight;
+  w->dev = d;
   w->shape.assign(shape, shape + ndim);
   w->numel = 1;
   for (size_t i = 0; i < ndim; i++) w->numel *= shape[i];
@@ -243,6 +244,7 @@ int tb200_alloc(tb200_device* d, size_t len, tb200_buffer** out) {
   if (int rc = use(d)) return rc;
   ARG_CHECK(out, "null output handle");
   auto* b = new tb200_buffer;
+  b->dev = d;
   b->len = b->cap = len;
   if (len) {
     cudaError_t e = cudaMalloc(&b->ptr, len * 4);

@@ -55,12 +55,14 @@ struct tb200_device {
 struct tb200_buffer {
   float* ptr = nullptr;
   size_t len = 0, cap = 0;
+  const tb200_device* dev = nullptr;  // that it was made on
 };
 
 struct tb200_weight {
   uint16_t* ptr = nullptr;
   std::vector<size_t> shape;
   size_t numel = 0;
+  const tb200_device* dev = nullptr;  // that it was made on
   bool has_map = false;
   CUtensorMap map{};  // operand map of a matrix for the tensor-core contraction
 };
@@ -73,6 +75,7 @@ struct tb200_q8 {
   float* scales = nullptr;   // [cap]
   size_t rows = 0, cap = 0, cols = 0;
   size_t ld = 0;  // cols rounded up to 16 bytes; the padding holds zeros
+  const tb200_device* dev = nullptr;  // that it was made on
 };
 
 struct FusedLayer {
@@ -192,6 +195,12 @@ int use(tb200_device* d);
 // Waits for the device's stream and reports an error that a kernel left in
 // async_err since the last such call.
 int settle(tb200_device* d);
+// Whether the operands, handles or null, were made on `d`: another device's
+// memory cannot be read from here, another stream's work is in no order with this one's.
+template <class... H>
+bool of(const tb200_device* d, const H*... h) {
+  return (... && (!h || h->dev == d));
+}
 // model.rs:239-250, on the host.
 std::vector<float> rope_table(size_t max_len, size_t head_dim, float theta);
 const char* last_error();
