@@ -384,6 +384,48 @@ def test_operands_of_another_device(b200):
     b200.sync()
 
 
+@pytest.mark.gpu
+def test_rows_past_32_bit_offsets(b200):
+    """2.2 M rows of 2048: 4.5 G values and 8-bit integers, products of up to 2.3 G values."""
+    torch = pytest.importorskip("torch")
+    rows, cols = 2200003, 2048
+    at = [0, 1048577, 2097153, rows - 1]
+    v = sample_rows(4, cols, 91)
+    x, q = b200.alloc(rows * cols), b200.q8(rows, cols)
+    for i, r in enumerate(at):
+        b200.copy(x, r * cols, buf(b200, v[i]), 0, cols)
+
+    def rows_at(q):
+        b200.sync()
+        return (torch.as_tensor(q.values, device="cuda")[at].cpu().numpy(),
+                torch.as_tensor(q.scales, device="cuda")[at].cpu().numpy())
+
+    b200.quantize(q, x)
+    for got, exp in zip(rows_at(q), ref_rows(v)):
+        same(got, exp)
+    wq, ws = rows_at(q)
+    b200.dequantize(x, q)
+    b200.sync()
+    same(torch.as_tensor(x, device="cuda").view(rows, cols)[at].cpu().numpy(), wq.astype(F32) * ws[:, None])
+    for i, r in enumerate(at):
+        b200.copy(x, r * cols, buf(b200, v[i]), 0, cols)
+    bits, w = bf16(np.random.default_rng(5).standard_normal(cols).astype(F32))
+    b200.add_rmsnorm_q8(q, x, None, b200.upload(tb.Tensor([cols], bits)), 1e-6)
+    for got, exp in zip(rows_at(q), ref_rows(ref_norm(v, None, w, 1e-6)[1])):
+        same(got, exp)
+    del x
+
+    wq, ws = rows_at(q)
+    out = b200.alloc(1030 * rows)
+    for tokens in (3, 20, 1000, 1030):
+        _, _, xq, xs = product_inputs(tokens, 1, cols, tokens)
+        b200.resize(out, tokens * rows)
+        b200.matmul_q8(out, q, rows_of(b200, xq, xs))
+        b200.sync()
+        got = torch.as_tensor(out, device="cuda").view(tokens, rows)[:, at].cpu().numpy()
+        same(got, ref_matmul(wq, ws, xq, xs))
+
+
 # ---- with torch, and captured --------------------------------------------------------------
 
 @pytest.mark.gpu
