@@ -268,6 +268,60 @@ def test_many_rows_that_are_not_ordinary(b200, vocab, top):
         assert np.all(np.abs(g[ok] - e[ok]) <= CHAIN * EPS * (2 + np.abs(e[ok])))
 
 
+FAR = [-1e10, -1e20, -1e30, 1e7, 1e10, 1e30]
+
+
+def far_rows(vocab, far):
+    """Rows whose first, last, or only logits lie at `far`: finite mask values where it is negative, maxima alone,
+    tied and a step apart where it is positive."""
+    rng = np.random.default_rng(vocab)
+    far, n = F32(far), min(vocab - 9, 4500)  # n: more than eight warps' first steps
+    x = rng.standard_normal((9, vocab)).astype(F32) * F32(2)
+    x[0, :n] = far
+    x[1, vocab - n:] = far
+    x[2] = far
+    x[3], x[3, vocab // 2] = far, 1.5
+    x[4], x[4, vocab - 5:] = far, x[5, :5]
+    x[5, ::3] = far
+    x[6, 7] = far
+    x[7, [3, vocab // 2, vocab - 1]] = far
+    x[8, 2:40:2], x[8, 1] = far, np.nextafter(far, F32(0))
+    return x
+
+
+def check_far(got, x, tokens, top, at):
+    """Tolerances: the sums' CHAIN for log Z (twice for the entropy, which has T / (1 + S) as well), and two roundings
+    relative to the result, which CHAIN covers too; see above. Exponents of shares that count are below 200, and
+    their one rounding moves a share by at most 2^-24 of its exponent."""
+    lp, ent, ids, tops = reference(x, tokens, top)
+    assert (got[2] == ids[at]).all()
+    for g, e in ((got[0], lp), (got[1], ent), (got[3], tops)):
+        e = e[at]
+        assert np.isfinite(e).all() and np.isfinite(g).all()
+        assert np.all(np.abs(g - e) <= 2 * CHAIN * EPS * (1 + np.abs(e)))
+
+
+# By a warp in registers, step by step, by CTAs for whole rows, for pieces, for runs that end inside rows.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,top", [(9, 500, 3), (9, 2045, 20), (1350, 5003, 0), (1350, 5003, 5),
+                                            (1800, 9001, 1), (9, 9001, 1), (9, 70001, 0), (9, 70001, 1),
+                                            (63, 151936, 5), (405, 40003, 3), (657, 40003, 1)])
+@pytest.mark.parametrize("far", FAR)
+def test_logits_far_from_zero(b200, rows, vocab, top, far):
+    """Magnitudes past 2^20, where steps of f32(m log2 e) are no small numbers: whole and half-masked rows, and maxima
+    with ties and neighbours."""
+    torch = pytest.importorskip("torch")
+    x = far_rows(vocab, far)
+    tokens = np.array([vocab - 1, 0, 5, vocab // 2, vocab - 1, 1, 7, 3, 2])
+    at = np.arange(rows) % 9
+    b = b200.alloc(rows * vocab)
+    b200.sync()
+    given = torch.as_tensor(x, device="cuda")[torch.as_tensor(at, device="cuda")]
+    torch.as_tensor(b, device="cuda").copy_(given.reshape(-1))
+    torch.cuda.synchronize()
+    check_far(tb.LogProbs(b200, rows, vocab, top).score(b, tokens[at]), x, tokens, top, at)
+
+
 @pytest.mark.gpu
 def test_rows_behind_the_last_stay(b200):
     """Fewer rows than the scorer holds; the same scorer again with others."""

@@ -146,6 +146,10 @@ struct Row {
 // A warp's set while it grows: m and own are the warp's, s and t each lane's
 // shares of the sums, taken at c = f32(m log2 e) in the place of m log2 e, which
 // saves an instruction a logit: what that leaves out (lo) is put right in settled().
+// A share holds 2^lo and settled() takes it out again, so lo has to be small: up
+// to |m| = 2^20 it is at most 2^-4, half a step of c there. Beyond (logits of a finite
+// mask value such as -1e10 or -1e30, where a step of c is hundreds and more) the
+// shares are taken at m itself, by a subtraction and a product.
 struct Running {
   float m, c, lo, s, t;
   int order;  // of m
@@ -155,10 +159,9 @@ struct Running {
     order = o;
     m = unorder(o);
     c = m * kLog2e;
-    lo = m > -INFINITY && !huge() ? fmaf(m, kLog2e, -c) : 0.f;
+    lo = m > -INFINITY && !far() ? fmaf(m, kLog2e, -c) : 0.f;
   }
-  // Whether m log2 e may be past f32's range.
-  __device__ __forceinline__ bool huge() const { return fabsf(m) > 1e38f; }
+  __device__ __forceinline__ bool far() const { return fabsf(m) > 0x1p20f; }
   __device__ __forceinline__ Soft settled() const {
     const float f = ex2(-lo);
     return Soft{m, s * f, fmaf(lo, s, t) * f, own ? 1.f : 0.f};
@@ -178,9 +181,9 @@ struct Running {
     }
   }
   // A logit's share of the sums. Far below the maximum (or excluded) it adds 0, not 0 * -inf.
-  template <bool HUGE>
+  template <bool FAR>
   __device__ __forceinline__ void add(float x) {
-    const float d = fmaxf(HUGE ? (x - m) * kLog2e : fmaf(x, kLog2e, -c), -200.0f);
+    const float d = fmaxf(FAR ? (x - m) * kLog2e : fmaf(x, kLog2e, -c), -200.0f);
     const float e = ex2(d);
     s += e;
     t = fmaf(-d, e, t);
@@ -242,7 +245,7 @@ __device__ __forceinline__ void step_add(Running& a, float (&x)[kStep][4], int l
         if (i == mine) x[i / 4][i % 4] = -INFINITY;
     }
   }
-  if (a.huge()) {
+  if (a.far()) {
     for (int i = 0; i < kStep * 4; i++) a.add<true>(x[i / 4][i % 4]);
     return;
   }
