@@ -323,6 +323,20 @@ def test_logits_far_from_zero(b200, rows, vocab, top, far):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(9, 2000), (1350, 5003), (9, 70001)])
+@pytest.mark.parametrize("base", [3e5, 9e5, 1.2e6, 5e6])
+def test_ordinary_rows_moved_far(b200, rows, vocab, base):
+    """Rows whose logits lie a few apart on both sides of the limit, on a coarse grid that f32 holds."""
+    rng = np.random.default_rng(int(base))
+    x = (np.round(rng.standard_normal((9, vocab)) * 6) / 2).astype(F32)
+    x[1::2] = -F32(base) + x[1::2]
+    x[::2] = F32(base) + x[::2]
+    at = np.arange(rows) % 9
+    tokens = rng.integers(0, vocab, 9)
+    check_far(tb.LogProbs(b200, rows, vocab, 4).score(buf(b200, x[at]), tokens[at]), x, tokens, 4, at)
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_last_stay(b200):
     """Fewer rows than the scorer holds; the same scorer again with others."""
     torch = pytest.importorskip("torch")

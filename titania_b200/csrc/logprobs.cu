@@ -166,12 +166,14 @@ struct Running {
     const float f = ex2(-lo);
     return Soft{m, s * f, fmaf(lo, s, t) * f, own ? 1.f : 0.f};
   }
-  // Refers the sums to a larger maximum; lane 0 takes the old one's own term.
+  // Refers the sums to a larger maximum; lane 0 takes the old one's own term. The
+  // old sums are brought to c, where the shares to come are taken: brought to m
+  // they were off by 2^lo, which is 1 + 5e-3 at m = 3e5.
   __device__ __forceinline__ void raise(int o, int lane) {
     const Soft old = settled();
     const int before = order;
     refer(o);
-    const float d = (m - old.m) * kLog2e, e = ex2(-d);
+    const float d = far() ? (m - old.m) * kLog2e : fmaf(-old.m, kLog2e, c), e = ex2(-d);
     if (before <= kNegInf || e == 0.0f) {
       s = old.s * 0.0f;  // a NaN stays
       t = 0.0f;
