@@ -234,8 +234,11 @@ TB200_API int tb200_add_rmsnorm_q8(tb200_device* dev, tb200_q8* out, tb200_buffe
  * tb200_matmul over 8-bit rows. The sum of integer products is exact (32-bit
  * integers; up to 131071 columns), its f32 value is then multiplied by the f32
  * product of the scales. out holds x.rows * w.rows values. An error inside
- * the kernel (a wait that timed out) is reported by the next call that waits
- * (tb200_sync, tb200_read). */
+ * the kernel (a wait that timed out) is TB200_ERR_TIMEOUT, once, from the next
+ * call on the device that waits for its work and hands out or takes values:
+ * tb200_sync, tb200_read, tb200_write, tb200_argmax, tb200_matmul of several
+ * tokens, tb200_q8_read, tb200_q8_write, tb200_sample, tb200_sampler_state,
+ * tb200_score. What that call returned is then not to be used. */
 TB200_API int tb200_matmul_q8(tb200_device* dev, tb200_buffer* out, const tb200_q8* w, const tb200_q8* x);
 
 /* The trait has no free (handles live as long as the process, as with

@@ -42,12 +42,16 @@ int use(tb200_device* d) {
   return TB200_OK;
 }
 
-int settle(tb200_device* d) {
-  CUDA_TRY(cudaStreamSynchronize(d->stream));
+int report(tb200_device* d) {
   volatile int* e = d->async_err;
   if (!*e) return TB200_OK;
   *e = 0;
   return fail(TB200_ERR_TIMEOUT, "a wait inside an 8-bit contraction timed out; its output is not complete");
+}
+
+int settle(tb200_device* d) {
+  CUDA_TRY(cudaStreamSynchronize(d->stream));
+  return report(d);
 }
 
 // model.rs:239-250, on the host exactly as the reference computes it.
@@ -133,7 +137,7 @@ int matmul_tokens(tb200_device* d, tb200_buffer* out, const tb200_weight* w, con
     cudaMemsetAsync(d->err, 0, sizeof(int), s);
     return fail(TB200_ERR_TIMEOUT, "matmul: a wait inside the contraction timed out");
   }
-  return TB200_OK;
+  return rt::report(d);
 }
 
 }  // namespace
@@ -285,8 +289,7 @@ int tb200_write(tb200_device* d, tb200_buffer* b, const float* data, size_t len)
   ARG_CHECK(b && (data || len == 0), "null argument");
   ARG_CHECK(len == b->len, "write: " + std::to_string(len) + " values into a buffer of " + std::to_string(b->len));
   if (len) CUDA_TRY(cudaMemcpyAsync(b->ptr, data, len * 4, cudaMemcpyHostToDevice, d->stream));
-  CUDA_TRY(cudaStreamSynchronize(d->stream));
-  return TB200_OK;
+  return rt::settle(d);
 }
 
 // cpu.rs:34-36 / titania.rs:139-143
@@ -433,7 +436,7 @@ int tb200_argmax(tb200_device* d, const tb200_buffer* logits, uint32_t* out) {
   if (int rc = launched("argmax")) return rc;
   unsigned long long key = 0;
   CUDA_TRY(cudaMemcpyAsync(&key, d->best, sizeof key, cudaMemcpyDeviceToHost, d->stream));
-  CUDA_TRY(cudaStreamSynchronize(d->stream));
+  if (int rc = rt::settle(d)) return rc;
   *out = 0xFFFFFFFFu - uint32_t(key & 0xFFFFFFFFu);
   return TB200_OK;
 }

@@ -192,8 +192,12 @@ int fail(int code, const std::string& msg);
 int launched(const char* what);
 // Makes `d` the current device.
 int use(tb200_device* d);
-// Waits for the device's stream and reports an error that a kernel left in
-// async_err since the last such call.
+// Reports an error that a kernel left in async_err since the last such call;
+// the device's stream has been waited for.
+int report(tb200_device* d);
+// Waits for the device's stream, then reports: how the calls end that wait and hand
+// out results or take values (those that make, load or free handles wait without
+// reporting, and leave the error for the next of these).
 int settle(tb200_device* d);
 // Whether the operands, handles or null, were made on `d`: another device's
 // memory cannot be read from here, another stream's work is in no order with this one's.

@@ -196,8 +196,7 @@ int tb200_sample(tb200_sampler* s, const tb200_buffer* logits, uint32_t* tokens)
   ARG_CHECK(tokens, "null argument");
   if (int rc = tb200_sample_enqueue(s, logits)) return rc;
   CUDA_TRY(cudaMemcpyAsync(tokens, s->tokens, s->rows * 4, cudaMemcpyDeviceToHost, s->dev->stream));
-  CUDA_TRY(cudaStreamSynchronize(s->dev->stream));
-  return TB200_OK;
+  return rt::settle(s->dev);
 }
 
 int tb200_sampler_state(tb200_sampler* s, uint64_t* out) {
@@ -205,7 +204,7 @@ int tb200_sampler_state(tb200_sampler* s, uint64_t* out) {
   if (int rc = rt::use(s->dev)) return rc;
   CUDA_TRY(cudaStreamSynchronize(s->dev->stream));
   CUDA_TRY(cudaMemcpy(out, s->state, s->rows * 8, cudaMemcpyDeviceToHost));
-  return TB200_OK;
+  return rt::report(s->dev);
 }
 
 }  // extern "C"
