@@ -622,6 +622,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
   if (warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory may go
   q_fence_before();
   __syncthreads();
+  // The first CTA's last commit arrives here too, which nothing above has waited for: not in shared memory that
+  // may be another kernel's by then.
+  if (CG == 2 && rank == 1 && warp == 1) mbar_wait(&tl.mdone, 0, nullptr);
   if constexpr (CG == 2 || SPLIT) cluster_sync();  // nothing reads or signals the other CTAs' memory any more
   if (warp == 1) {
     q_fence_after();
