@@ -490,6 +490,39 @@ def test_captured_chain(b200, tokens):
         check(call)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 8, 40])
+def test_operands_written_by_the_kernel_before(b200, tokens):
+    """Each kernel starts while the one that writes its input still runs: two inputs in turns through the same
+    buffers, nothing waited for, and every result as when it is computed alone."""
+    torch = pytest.importorskip("torch")
+    cols, channels = 1024, 1500
+    wq, ws, _, _ = product_inputs(1, channels, cols, tokens)
+    w, ids = rows_of(b200, wq, ws), torch.arange(tokens, dtype=torch.int32, device="cuda")
+    x = [buf(b200, np.random.default_rng(i).standard_normal((tokens, cols)).astype(F32)) for i in range(2)]
+    q, out, back = b200.q8(tokens, cols), b200.alloc(tokens * channels), b200.alloc(tokens * cols)
+    lp = tb.LogProbs(b200, tokens, channels, 5)
+    torch.cuda.synchronize()
+
+    def chain(i):
+        b200.quantize(q, x[i])
+        b200.dequantize(back, q)
+        b200.quantize(q, back)
+        b200.matmul_q8(out, w, q)
+        lp.enqueue(out, ids)
+        with torch.cuda.stream(torch.cuda.ExternalStream(b200.stream)):
+            return [torch.as_tensor(a, device="cuda").clone() for a in (out, lp.logprob, lp.top_ids)]
+
+    alone = []
+    for i in range(2):
+        alone.append(chain(i))
+        b200.sync()
+    assert not torch.equal(alone[0][0], alone[1][0])
+    for i, got in [(n % 2, chain(n % 2)) for n in range(60)]:
+        b200.sync()
+        assert all(torch.equal(g, a) for g, a in zip(got, alone[i]))
+
+
 # ---- a whole model --------------------------------------------------------------------------
 
 class Checked:

@@ -128,6 +128,38 @@ __device__ __forceinline__ void set_error(int* err, int code) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads of what the kernel before this one may have written. A `const __restrict__`
+// operand or __ldg would promise that nothing writes it while this kernel runs, which
+// begins before that one has ended; a plain load keeps its place among this kernel's
+// stores and barriers. These are coherent loads that the compiler may move, but not
+// above pdl_wait(): their addresses come from a pointer that after_wait() gives.
+template <class T>
+__device__ __forceinline__ T* after_wait(T* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+__device__ __forceinline__ float ld_f32(const float* p) {
+  float v;
+  asm("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ld_f32x4(const float* p) {
+  float4 v;
+  asm("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int4 ld_s32x4(const int4* p) {
+  int4 v;
+  asm("ld.global.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// The same for what is read once.
+__device__ __forceinline__ int4 ld_stream_s32x4(const int4* p) {
+  int4 v;
+  asm("ld.global.cs.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // Launches a kernel that begins with pdl_wait() so that it may start early.
 template <class... Params, class... Args>
 inline void launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {

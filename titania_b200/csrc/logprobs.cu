@@ -129,7 +129,7 @@ struct Row {
   // Element i of the row for value j of lane's granule of block b, or out of range.
   __device__ __forceinline__ int element(int b, int lane, int j) const { return b * kBlock + 4 * lane + j - shift; }
   __device__ __forceinline__ float4 load(int b, int lane) const {
-    return __ldg(reinterpret_cast<const float4*>(base) + size_t(b) * 32 + lane);
+    return ld_f32x4(base + size_t(b) * kBlock + 4 * lane);
   }
   // A block at the row's end: `fill` in the place of what is not the row's.
   __device__ __forceinline__ float4 load_end(int b, int lane, float fill) const {
@@ -137,7 +137,7 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int i = element(b, lane, j);
-      v[j] = i >= 0 && i < vocab ? __ldg(base + size_t(b) * kBlock + 4 * lane + j) : fill;
+      v[j] = i >= 0 && i < vocab ? ld_f32(base + size_t(b) * kBlock + 4 * lane + j) : fill;
     }
     return make_float4(v[0], v[1], v[2], v[3]);
   }
@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
   __shared__ ScoreShared sh;
   pdl_launch_dependents();
   pdl_wait();
+  a.logits = after_wait(a.logits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float nan = __int_as_float(0x7FC00000);
   long long g = blockIdx.x * a.run;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_score(ScoreArgs a) {
     float given = nan;
     if (threadIdx.x == 0) {
       const uint32_t tok = a.tokens[row];
-      if (tok < uint32_t(a.vocab)) given = __ldg(r.base + r.shift + tok);
+      if (tok < uint32_t(a.vocab)) given = ld_f32(r.base + r.shift + tok);
     }
     int st = s0 + warp;
     bool whole = false;
@@ -640,6 +641,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) k_alternatives(ScoreArgs a) 
   __shared__ ScoreShared sh;
   pdl_launch_dependents();
   pdl_wait();
+  a.logits = after_wait(a.logits);
   const size_t row = blockIdx.x;
   const Row r(a.logits, row, a.vocab);
   int entry[kOwn];
@@ -656,13 +658,14 @@ template <int S>
 __global__ void __launch_bounds__(kScoreThreads) k_score_rows(ScoreArgs a, int rows) {
   pdl_launch_dependents();
   pdl_wait();
+  a.logits = after_wait(a.logits);
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * kScoreWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const Row r(a.logits, size_t(row), a.vocab);
   const float nan = __int_as_float(0x7FC00000);
   const uint32_t tok = a.tokens[row];
-  const float given = tok < uint32_t(a.vocab) ? __ldg(r.base + r.shift + tok) : nan;
+  const float given = tok < uint32_t(a.vocab) ? ld_f32(r.base + r.shift + tok) : nan;
   float x[S][kStep][4], met = 0.f;
   int top[S], common = INT_MIN;
 #pragma unroll
@@ -799,13 +802,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_score_long_rows(ScoreArgs a,
   __shared__ unsigned long long rooms[kRowWarps][kRoom];
   pdl_launch_dependents();
   pdl_wait();
+  a.logits = after_wait(a.logits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * kRowWarps + warp;
   if (row >= rows) return;
   const Row r(a.logits, size_t(row), a.vocab);
   const float nan = __int_as_float(0x7FC00000);
   const uint32_t tok = a.tokens[row];
-  const float given = tok < uint32_t(a.vocab) ? __ldg(r.base + r.shift + tok) : nan;
+  const float given = tok < uint32_t(a.vocab) ? ld_f32(r.base + r.shift + tok) : nan;
   auto whole = [&](int st) { return r.inside(st * kStep) && r.inside(st * kStep + kStep - 1); };
   auto fetch = [&](int st, float4 (&v)[kStep]) {
     const bool w = whole(st);

@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(1024) k_long_rows_q8(RowArgs a) {
 // a thread, so that a thread has more than one word on its way; blockDim.x
 // threads along a row, blockDim.y rows.
 constexpr int kDeq = 4;
-__global__ void __launch_bounds__(256) k_dequantize(float* __restrict__ out, const int8_t* __restrict__ q,
-                                                    const float* __restrict__ scale, long long rows, int cols, int ld) {
+__global__ void __launch_bounds__(256) k_dequantize(float* out, const int8_t* q, const float* scale, long long rows,
+                                                    int cols, int ld) {
   pdl_launch_dependents();
   pdl_wait();
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
