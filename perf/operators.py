@@ -29,12 +29,15 @@ _device = None
 
 
 def _dev():
-    """The framework's device, opened once."""
+    """The framework's device, opened once. Its stream becomes torch's current one, so that what torch does with
+    the operators' inputs and outputs, which share the framework's memory, stands in order with them."""
     global _device
     if _device is None:
         import titania_b200
 
         _device = titania_b200.B200(torch.cuda.current_device())
+    if torch.cuda.current_stream().cuda_stream != _device.stream:
+        torch.cuda.set_stream(torch.cuda.ExternalStream(_device.stream))
     return _device
 
 
@@ -143,6 +146,8 @@ def _view(array):
 
 
 def prepare(case, seed):
+    if own:
+        _dev()
     state = _inputs(case, seed)
     state["op"] = case["op"]
     if case["op"] == "logprobs":
