@@ -29,7 +29,7 @@
 // maxima (each of those has an element at least as large as any element of
 // another block), so only those are read again. In k_score that is a few
 // microseconds a row, of waiting more than of work: with few rows the CTA that
-// finishes a row does it (64 rows, five alternatives: 15.8 us, 11.5 with none),
+// finishes a row does it (64 rows, five alternatives: 15.8 us, 11.5 with none, in L2; 17.4 and 13.5 from memory),
 // with many it is a kernel of its own with a CTA for every row (1111 rows: 124 us;
 // in one kernel 131). One alternative is the maximum itself, whose place the warps
 // keep (112 us).
@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(kScoreThreads) k_score_rows(ScoreArgs a, int r
 // blocks of every step: k of the sets' largest logits are at least the k-th of
 // them, which bounds the k-th logit from below closely (about 1.4 k logits reach it at
 // k = 64). The blocks that reach it, by their maxima, are read again. 2048 x 5000, us,
-// no and twenty alternatives: 10.2 and 19.7, by k_score and k_alternatives 17.2 and 48.1.
+// no and twenty alternatives: 10.2 and 19.7, by k_score and k_alternatives 17.2 and 48.1 (from memory 11.5 and 21.0).
 constexpr int kRowSteps = 64;
 constexpr int kRowWarps = 4;
 constexpr int kRoom = 256;  // candidates that a warp holds

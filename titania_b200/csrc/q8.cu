@@ -7,11 +7,14 @@
 //   tb200_quantize_weight  n = w (bf16), a row per output channel
 //   tb200_add_rmsnorm_q8   h = f32(x + y), stored back to x;
 //                          n = h * w / sqrt(mean(h^2) + eps)
-// All of it after the f32 addition is 64-bit arithmetic. h * w (24 + 8 bits) and
-// h^2 (48 bits) are exact there, so which integer a value next to the middle of
-// two becomes does not depend on the order of a sum, on the number of threads
-// or on how a compiler contracts a product: the rows are the same, bit for
-// bit, whatever variant runs, and equal those of any 64-bit restatement.
+// All of it after the f32 addition is 64-bit arithmetic, in which h * w (24 + 8
+// bits) and h^2 (48 bits) are exact. Rows of f32 and bf16 are therefore the same,
+// bit for bit, whatever variant runs, and equal those of any 64-bit restatement. A
+// norm's sum of squares is rounded in an order that the variant sets (the numbers of
+// rows and columns choose it), and its mean and square root round once each: the row's
+// factor agrees with another order's to a few times 1e-15 (up to 16384 columns; the
+// bound grows with them), so only a value that near to the middle of two integers, or a scale
+// that near to the middle of two f32 values, may come out as the other one.
 #include <algorithm>
 #include <string>
 
@@ -122,7 +125,7 @@ __host__ __device__ constexpr int row_threads(int e) { return e == 8 ? 512 : e =
 //
 // Every warp of a row repeats what a row costs beside its values (the two
 // reductions, the constants): 5003 x 2560 with the residual takes 46, 33 and
-// 30 us with one, two and four groups a thread.
+// 30 us with one, two and four groups a thread (31.4 over several buffers in turns, 5.3 TB/s).
 //
 // What should bound it is memory, so the 64-bit work is kept small (with all of
 // it in 64 bits the kernel took 51 instructions a value): only the sum of
@@ -323,7 +326,7 @@ __global__ void __launch_bounds__(1024) k_long_rows_q8(RowArgs a) {
 
 // Groups of four values (the aligned ones of the output, whose
 // rows begin `shift` values after one where `cols` is no multiple of four: an
-// unaligned store4 each took 5000 x 2562 from 10.7 to 22 us), kDeq of them
+// unaligned store4 each took 5000 x 2562 from 10.7 to 22 us in L2; from memory 16.2), kDeq of them
 // a thread, so that a thread has more than one word on its way; blockDim.x
 // threads along a row, blockDim.y rows.
 constexpr int kDeq = 4;
@@ -371,8 +374,8 @@ void launch_rows_q8(tb200_device* d, const RowArgs& a, size_t rows) {
   const int groups = a.ld / 4;  // of four values; the padding is theirs too
   // Few rows: as many threads on each as it has groups, since what counts is how
   // long one row takes. Many: as few warps as can hold it, one if it fits, up to
-  // four groups a thread with a norm, eight without (2048 x 9728: 31 and 17 us with
-  // four and eight; with the residual and the norm 54 and 83, for want of registers).
+  // four groups a thread with a norm, eight without (2048 x 9728, one buffer: 31 and 17 us with
+  // four and eight, 18.9 from memory; with the residual and the norm 54 and 83, for want of registers).
   int e = 1;
   if (rows >= size_t(2 * d->sms))
     while (e < (kNorm ? 4 : 8) && groups > e * 32) e *= 2;

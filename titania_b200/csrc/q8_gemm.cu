@@ -798,7 +798,7 @@ int tb200_matmul_q8(tb200_device* d, tb200_buffer* out, const tb200_q8* w, const
   if (!x->rows || !w->rows) return TB200_OK;
   // Three to eight tokens over many weights keep the CUDA cores busy for longer than the weights take to arrive
   // (us there and on the tensor cores: four tokens, 2560 x 9728 8.4 and 9.4, 151936 x 1024 33.6 and 28.1; eight,
-  // 1024 x 2048 3.0 and 4.9, 2560 x 4096 5.9 and 6.9, 9728 x 2560 9.9 and 7.9), but few channels make few tiles
+  // 1024 x 2048 2.1 and 4.9, 2560 x 4096 6.0 and 6.9, 9728 x 2560 9.9 and 7.9), but few channels make few tiles
   // (eight tokens, 1000 x 20000 7.2 and 12.3).
   const bool few = w->rows <= size_t(8) * d->sms;
   if (x->rows > 8 || (x->rows > 2 && !few && x->rows * w->rows * w->cols > size_t(128) << 20))
