@@ -523,6 +523,36 @@ def test_operands_written_by_the_kernel_before(b200, tokens):
         assert all(torch.equal(g, a) for g, a in zip(got, alone[i]))
 
 
+@pytest.mark.gpu
+def test_two_devices_at_once(b200):
+    """Products of every kind and scores on two handles' streams, nothing waited for between them."""
+    torch = pytest.importorskip("torch")
+    other = tb.B200(0)
+    shapes = [(1, 4096, 1024), (5, 1000, 4000), (40, 2000, 1024), (64, 512, 9728), (300, 1200, 1100), (1100, 640, 2176)]
+    work = []
+    for k, dev in enumerate((b200, other)):
+        for tokens, channels, cols in shapes:
+            wq, ws, xq, xs = product_inputs(tokens, channels, cols, tokens + k)
+            lp = tb.LogProbs(dev, tokens, channels, 3)
+            work.append((dev, rows_of(dev, wq, ws), rows_of(dev, xq, xs), dev.alloc(tokens * channels), lp,
+                         torch.arange(tokens, dtype=torch.int32, device="cuda") % channels, ref_matmul(wq, ws, xq, xs)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for dev, w, x, out, lp, ids, _ in work:
+            dev.matmul_q8(out, w, x)
+            lp.enqueue(out, ids)
+    b200.sync()
+    other.sync()
+    for dev, _, _, out, lp, ids, exp in work:
+        same(dev.read(out).reshape(exp.shape), exp)
+        now = [torch.as_tensor(a, device="cuda").clone() for a in (lp.logprob, lp.entropy, lp.top_ids)]
+        torch.cuda.synchronize()
+        lp.enqueue(out, ids)
+        dev.sync()
+        assert all(torch.equal(torch.as_tensor(a, device="cuda"), b)
+                   for a, b in zip((lp.logprob, lp.entropy, lp.top_ids), now))
+
+
 # ---- a whole model --------------------------------------------------------------------------
 
 class Checked:
